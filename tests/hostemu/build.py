@@ -19,7 +19,7 @@ ROOT = HERE.parent.parent
 CSRC = ROOT / "yolo_master_amd" / "csrc"
 OUT = HERE / "_build"
 SOURCES = ["mixture.hip", "mixattn.hip", "conv_glds.hip", "post.hip", "preproc.hip", "mlp.hip", "stem2.hip", "c3k2f.hip", "detcls.hip",
-           "esmoe.hip", "attn.hip", "nms.hip", "conv.hip", "dwconv.hip", "elementwise.hip", "capi.hip"]
+           "esmoe.hip", "attn.hip", "nms.hip", "conv.hip", "dwconv.hip", "elementwise.hip", "capi.hip", "rmsnorm.hip", "tokens.hip", "expert.hip"]
 
 
 @contextlib.contextmanager
@@ -53,7 +53,7 @@ def build(force: bool = False, f16: bool = False) -> Path | None:
 def _build_locked(cxx, force: bool, f16: bool) -> Path:
     lib = OUT / ("libymk_hostemu_f16.so" if f16 else "libymk_hostemu.so")
     srcs = [CSRC / s for s in SOURCES]
-    deps = srcs + [CSRC / "ymk_common.h", CSRC / "glds.h", CSRC / "igemm.h", ROOT / "include" / "ymk_mixture.h", HERE / "hip" / "hip_runtime.h", Path(__file__)]
+    deps = srcs + [CSRC / "ymk_common.h", CSRC / "glds.h", CSRC / "igemm.h", ROOT / "include" / "ymk_mixture.h", ROOT / "include" / "ymk_tokens.h", HERE / "hip" / "hip_runtime.h", Path(__file__)]
     if not force and lib.exists() and lib.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
         return lib
     units = []
@@ -66,6 +66,7 @@ def _build_locked(cxx, force: bool, f16: bool) -> Path:
         txt = txt.replace('#include "igemm.h"', f'#include "{CSRC / "igemm.h"}"')
         txt = txt.replace('#include "glds.h"', f'#include "{CSRC / "glds.h"}"')
         txt = txt.replace('#include "../../include/ymk_mixture.h"', f'#include "{ROOT / "include" / "ymk_mixture.h"}"')
+        txt = txt.replace('#include "../../include/ymk_tokens.h"', f'#include "{ROOT / "include" / "ymk_tokens.h"}"')
         u = OUT / (s.stem + ("_host_f16.cpp" if f16 else "_host.cpp"))
         u.write_text(txt)
         units.append(str(u))

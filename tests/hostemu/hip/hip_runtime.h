@@ -259,6 +259,89 @@ static inline hostemu_f32x4 __builtin_amdgcn_mfma_f32_16x16x4f32(float a, float 
     hostemu::wave_sync();
     return c;
 }
+// The 32x32 forms: lane l holds row l % 32 of its operand, elements (l / 32) * n .. + n - 1 of K (n elements a lane); D[(r / 4) * 8 + (l / 32) * 4 + r % 4][l % 32],
+// r = 0..15 (CDNA3/4 ISA; for the 64-deep 8-bit form the order of K is the operands' own, the same for both).
+typedef float hostemu_f32x16 __attribute__((ext_vector_type(16)));
+typedef int hostemu_i32x8 __attribute__((ext_vector_type(8)));
+namespace hostemu {
+inline float mfma_wide_a[MAX_LANES][32], mfma_wide_b[MAX_LANES][32];
+inline hostemu_f32x16 mfma32(int n, hostemu_f32x16 c) {   // operands published by the caller
+    const unsigned w0 = cur & ~63u, l = cur & 63u;
+    wave_sync();
+    for (int r = 0; r < 16; ++r) {
+        const unsigned i = (r / 4) * 8 + (l / 32) * 4 + r % 4, j = l % 32;
+        float s = 0.f;
+        for (unsigned h = 0; h < 2; ++h)
+            for (int e = 0; e < n; ++e) s += mfma_wide_a[w0 + h * 32 + i][e] * mfma_wide_b[w0 + h * 32 + j][e];
+        c[r] += s;
+    }
+    wave_sync();
+    return c;
+}
+// OCP e4m3: bias 7, subnormals at 2^-9, 0x7f / 0xff NaN, no infinities
+inline float from_e4m3(unsigned v) {
+    const int e = (v >> 3) & 15, m = v & 7;
+    if (e == 15 && m == 7) return __builtin_nanf("");
+    const float a = e ? std::ldexp((float)(8 + m), e - 10) : std::ldexp((float)m, -9);
+    return v & 0x80 ? -a : a;
+}
+inline unsigned to_e4m3(float f) {   // round to nearest even; beyond 464 NaN, as the hardware's conversion without clamping gives
+    const unsigned s = std::signbit(f) ? 0x80u : 0u;
+    const float a = std::fabs(f);
+    if (!(a <= 464.f)) return s | 0x7fu;
+    if (a >= 448.f) return s | 0x7eu;
+    int e;
+    std::frexp(a, &e);
+    const int q = a < std::ldexp(1.f, -6) ? -9 : e - 4;   // exponent of one step
+    const float n = std::nearbyint(std::ldexp(a, -q));    // 0..16 steps
+    if (a < std::ldexp(1.f, -6)) return s | (unsigned)n;  // 8 steps are the smallest normal number
+    unsigned m = (unsigned)n, ex = (unsigned)(q + 10);
+    if (m == 16) { m = 8; ++ex; }
+    return s | (ex << 3) | (m - 8);
+}
+}  // namespace hostemu
+static inline hostemu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_bf16(hostemu_bf16x8 a, hostemu_bf16x8 b, hostemu_f32x16 c, int, int, int) {
+    for (int e = 0; e < 8; ++e) { hostemu::mfma_wide_a[hostemu::cur][e] = (float)a[e]; hostemu::mfma_wide_b[hostemu::cur][e] = (float)b[e]; }
+    return hostemu::mfma32(8, c);
+}
+static inline hostemu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_f16(hostemu_f16x8 a, hostemu_f16x8 b, hostemu_f32x16 c, int, int, int) {
+    for (int e = 0; e < 8; ++e) { hostemu::mfma_wide_a[hostemu::cur][e] = (float)a[e]; hostemu::mfma_wide_b[hostemu::cur][e] = (float)b[e]; }
+    return hostemu::mfma32(8, c);
+}
+static inline hostemu_f32x16 __builtin_amdgcn_mfma_f32_32x32x2f32(float a, float b, hostemu_f32x16 c, int, int, int) {
+    hostemu::mfma_wide_a[hostemu::cur][0] = a;
+    hostemu::mfma_wide_b[hostemu::cur][0] = b;
+    return hostemu::mfma32(1, c);
+}
+static inline hostemu_f32x16 __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(hostemu_i32x8 a, hostemu_i32x8 b, hostemu_f32x16 c, int fmt_a, int fmt_b, int, int, int, int) {
+    if (fmt_a || fmt_b) abort();   // e4m3 only
+    for (int e = 0; e < 32; ++e) {
+        hostemu::mfma_wide_a[hostemu::cur][e] = hostemu::from_e4m3(((unsigned)a[e / 4] >> (e % 4 * 8)) & 255u);
+        hostemu::mfma_wide_b[hostemu::cur][e] = hostemu::from_e4m3(((unsigned)b[e / 4] >> (e % 4 * 8)) & 255u);
+    }
+    return hostemu::mfma32(32, c);
+}
+static inline int __builtin_amdgcn_cvt_pk_fp8_f32(float x, float y, int old, bool high) {
+    const unsigned v = hostemu::to_e4m3(x) | (hostemu::to_e4m3(y) << 8);
+    return (int)(high ? ((unsigned)old & 0xffffu) | (v << 16) : ((unsigned)old & 0xffff0000u) | v);
+}
+// ds_read_b64_tr_b16: the 16 lanes of a group read four rows of 16 16-bit elements, lane i the elements 4 (i % 4) .. + 3 of row i / 4 at its own
+// address, and lane i receives column i of them
+static inline hostemu_u32x2 hostemu_ds_read_tr16_b64(const char* p) {
+    uint64_t mine;
+    std::memcpy(&mine, p, 8);
+    const unsigned i = hostemu::cur & 15u;
+    uint64_t out = 0;
+    for (unsigned r = 0; r < 4; ++r) {
+        const uint64_t v = hostemu::exchange(mine, [&](unsigned l) { return (l & ~15u) + r * 4 + i / 4; });
+        out |= ((v >> (i % 4 * 16)) & 0xffffull) << (r * 16);
+    }
+    hostemu_u32x2 r;
+    r.x = (unsigned)out;
+    r.y = (unsigned)(out >> 32);
+    return r;
+}
+static inline int __ffsll(unsigned long long v) { return __builtin_ffsll((long long)v); }
 // LDS-DMA: 16 bytes per lane from the lane's global address to (wave-uniform LDS base) + lane * 16.  Completes at once
 // here, so counted-vmcnt mistakes are invisible; addressing, swizzles and masks are not.
 static inline void hostemu_global_load_lds16(const void* g, void* lds_base) {

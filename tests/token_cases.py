@@ -1,0 +1,394 @@
+"""Cases and 64-bit checks of the token operators (include/ymk_tokens.h), shared by tests/test_hostemu_tokens.py (CPU lane emulator) and
+tests/test_gpu_tokens.py.  Tolerances: u = 2^-24 is half a step of fp32, `half(t)` half a step of the stored type (relative), and a sum of n fp32
+terms is off by at most (its longest chain of additions) * u * (the sum of the terms' magnitudes)."""
+import torch
+
+U = 2.0**-24
+TINY = {torch.float32: 2.0**-150, torch.bfloat16: 2.0**-134, torch.float16: 2.0**-25}   # half a step of the subnormals
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rows_of(g, M, C, dtype, pad=0, dev="cpu", scale=1.0):
+    """[M, C] view with `pad` extra columns of NaN behind every row."""
+    buf = torch.full((max(M, 1), C + pad), float("nan"), dtype=dtype)
+    buf[:, :C] = (torch.randn((max(M, 1), C), generator=g) * scale).to(dtype)
+    return buf.to(dev)[:M, :C]
+
+
+def close(got, want, tol, what):
+    got, want, tol = got.double().cpu(), want.double().cpu(), tol.double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got - want).abs() <= tol)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() / tol.clamp_min(1e-300))[bad].max()):.3g} x the tolerance"
+
+
+# ------------------------------------------------------------------------------------------------------------------ norm
+# rows, channels, padding of the rows, residual
+NORMS = [(1, 1, 0, True), (3, 8, 0, True), (5, 33, 0, False), (70, 64, 8, True), (17, 100, 3, True), (2, 513, 0, True), (9, 1021, 0, True), (3, 2048, 8, True),
+         (2, 2056, 0, False), (600, 40, 0, True), (513, 24, 1, True), (0, 16, 0, True)]
+
+
+def check_norm(ops, dtype, case, dev="cpu", eps=1e-5):
+    M, C, pad, res = case
+    g = gen(M * 31 + C)
+    x, r = rows_of(g, M, C, dtype, pad, dev), rows_of(g, M, C, dtype, 0, dev) if res else None
+    w = (1 + 0.3 * torch.randn(C, generator=g)).to(dev)
+    y, h, rstd = ops.rms_norm(x, w, eps, residual=r)
+    want_h = (x.float() + r.float()).to(dtype) if res else x
+    assert torch.equal(h, want_h) and h.dtype == y.dtype == dtype
+    h64 = want_h.double().cpu()
+    r64 = 1 / (h64.square().mean(-1) + eps).sqrt()
+    # longest chain: 32 terms a lane, 10 levels of the tree; half of it reaches the root, and a handful of single roundings follow
+    rel = 40 * U
+    close(rstd, r64, r64 * rel, "rstd")
+    y64 = h64 * r64[:, None] * w.double().cpu()
+    close(y, y64, y64.abs() * (half(dtype) * (1 + rel) + rel) + TINY[dtype], "y")
+    q, scale, h2 = ops.rms_norm_quant(x, w, eps, residual=r)
+    assert torch.equal(h2, want_h) and q.dtype == torch.float8_e4m3fn and scale.dtype == torch.float32
+    top = y64.abs().amax(-1) if M else y64.new_zeros(0)
+    close(scale, top / 448, top / 448 * rel, "scale")
+    s = scale.double().cpu()[:, None]
+    q64 = q.cpu().double()
+    close(q64 * s, y64, torch.maximum(2.0**-4 * y64.abs(), 2.0**-10 * s) * (1 + 2.0**-12) + 2 * rel * y64.abs(), "q")
+    assert not M or bool((q64.abs().amax(-1) == 448).all())
+    # gradient
+    dy, dres = rows_of(g, M, C, dtype, pad, dev), rows_of(g, M, C, dtype, 0, dev)
+    dx, dw = ops.rms_norm_backward(dy, h, w, rstd, dres=dres)
+    d64, n64, w64 = dy.double().cpu(), h64 * r64[:, None], w.double().cpu()
+    g64 = d64 * w64
+    gn, gn_abs = ((g64 * n64).mean(-1, keepdim=True), (g64 * n64).abs().mean(-1, keepdim=True)) if M else (g64, g64)
+    rr = r64[:, None]
+    want = rr * (g64 - n64 * gn) + dres.double().cpu()
+    parts = rr * (g64.abs() + n64.abs() * gn_abs) + dres.double().cpu().abs()
+    close(dx, want, parts * (120 * U) + want.abs() * half(dtype) + TINY[dtype], "dx")
+    # a lane's rows, the groups of a workgroup, the partial rows of the workgroups: fewer than 256 additions in a chain for these sizes and for
+    # the largest (200000 rows: 49 a lane, 32 groups, 64 partial rows a strand, 16 strands); rstd's own error comes on top
+    close(dw, (d64 * n64).sum(0), (d64 * n64).abs().sum(0) * ((256 + 40) * U) + 1e-30, "dweight")
+    dx2, none = ops.rms_norm_backward(dy, h, w, rstd, need_dweight=False)
+    assert none is None
+    close(dx2, want - dres.double().cpu(), (parts - dres.double().cpu().abs()) * (120 * U) + want.abs() * half(dtype) + dres.double().cpu().abs() * half(dtype) + TINY[dtype], "dx alone")
+
+
+def check_norm_in_place(ops, dtype, dev="cpu"):
+    """The residual stream updated where it lies: h over residual, and over x."""
+    g = gen(5)
+    for C in (40, 37, 2100):
+        x, r = rows_of(g, 7, C, dtype, 0, dev), rows_of(g, 7, C, dtype, 0, dev)
+        w = torch.ones(C, device=dev)
+        y, h, _ = ops.rms_norm(x, w, residual=r)
+        x1, r1 = x.clone(), r.clone()
+        y1, h1, _ = ops.rms_norm(x1, w, residual=r1, residual_out=r1)
+        assert h1 is r1 and torch.equal(r1, h) and torch.equal(y1, y) and torch.equal(x1, x)
+        q2, s2, h2 = ops.rms_norm_quant(x1, w, residual=r, residual_out=x1)
+        assert h2 is x1 and torch.equal(x1, h)
+
+
+def check_norm_special(ops, dtype, dev="cpu"):
+    """All-zero rows, rows with NaN or infinity, rows of the type's smallest values; their neighbours are untouched by them."""
+    C = 72
+    x = torch.ones(6, C, dtype=dtype, device=dev)
+    x[1] = 0
+    x[2, 5] = float("nan")
+    x[3, 7] = float("inf")
+    x[4] = torch.finfo(dtype).tiny
+    w = torch.ones(C, device=dev)
+    q, s, _ = ops.rms_norm_quant(x, w, 0.0 if dtype == torch.float32 else 1e-6)
+    q, s = q.float().cpu(), s.cpu()
+    one = 1.0 if dtype == torch.float32 else float((1 / torch.tensor(1.0 + 1e-6)).sqrt())
+    for r in (0, 5):
+        assert bool((q[r] == 448).all()) and abs(float(s[r]) - one / 448) < 1e-6
+    if dtype != torch.float32:
+        assert float(s[1]) == 1.0 and bool((q[1] == 0).all())
+    assert bool(torch.isnan(s[2:4]).all()) and bool(torch.isnan(q[2:4]).all())
+    y, _, _ = ops.rms_norm(x, w, 1e-6)
+    y = y.float().cpu()
+    assert bool((y[1] == 0).all()) and bool(torch.isnan(y[2]).all()) and bool(torch.isnan(y[3, 7])) and bool(torch.isfinite(y[[0, 4, 5]]).all())
+
+
+def check_norm_differences(ops, dev="cpu"):
+    """<dx, u> and <dweight, v> against central differences of the forward."""
+    g = gen(9)
+    M, C, eps, d = 4, 48, 1e-5, 2.0**-6
+    x, dy = rows_of(g, M, C, torch.float32, 0, dev), rows_of(g, M, C, torch.float32, 0, dev)
+    w = (1 + 0.3 * torch.randn(C, generator=g)).to(dev)
+    u, v = torch.randn(M, C, generator=g).to(dev), torch.randn(C, generator=g).to(dev)
+    loss = lambda x_, w_: float((ops.rms_norm(x_, w_, eps)[0].double() * dy.double()).sum())   # noqa: E731
+    _, h, rstd = ops.rms_norm(x, w, eps)
+    dx, dw = ops.rms_norm_backward(dy, h, w, rstd)
+    # truncation d^2 / 6 times a third derivative of order one a row and unit direction (|u| ~ 7 a row), plus rounding u |L| / d
+    assert abs((loss(x + d * u, w) - loss(x - d * u, w)) / (2 * d) - float((dx.double() * u.double()).sum())) < 0.05
+    assert abs((loss(x, w + d * v) - loss(x, w - d * v)) / (2 * d) - float((dw.double() * v.double()).sum())) < 0.01
+
+
+# ---------------------------------------------------------------------------------------------------------------- tokens
+# tokens, top_k, experts, share without an expert, int64 indexes
+SORTS = [(0, 2, 4, 0.0, False), (1, 1, 1, 0.0, False), (1, 2, 8, 0.0, True), (5, 3, 7, 0.4, False), (300, 2, 16, 0.0, False), (257, 16, 255, 0.1, True), (64, 1, 256, 1.0, False),
+         (4096, 2, 3, 0.0, False), (4097, 2, 5, 0.3, True), (9001, 1, 64, 0.05, False), (5000, 3, 256, 0.5, False), (8200, 1, 1, 0.5, False)]
+
+
+def make_idx(g, T, K, E, dropped, wide):
+    idx = torch.randint(0, E, (T, K), generator=g)
+    gone = torch.rand(T, K, generator=g) < dropped
+    bad = torch.tensor([-1, E, -2**31, E + 7] + ([2**40, -2**40 + 1] if wide else []))
+    idx = torch.where(gone, bad[torch.randint(0, len(bad), (T, K), generator=g)], idx)
+    return idx if wide else idx.to(torch.int32)
+
+
+def sort_oracle(idx, E):
+    flat = idx.reshape(-1).long()
+    key = torch.where((flat >= 0) & (flat < E), flat, E)
+    order = torch.argsort(key, stable=True)
+    n = int((key < E).sum())
+    src = torch.full((flat.numel(),), -1, dtype=torch.int32)
+    src[:n] = order[:n].to(torch.int32)
+    row = torch.full((flat.numel(),), -1, dtype=torch.int32)
+    row[order[:n]] = torch.arange(n, dtype=torch.int32)
+    offsets = torch.zeros(E + 1, dtype=torch.int32)
+    offsets[1:] = torch.bincount(key, minlength=E + 1)[:E].cumsum(0).to(torch.int32)
+    return offsets, src, row.reshape(idx.shape), n
+
+
+def check_sort(ops, case, dev="cpu"):
+    T, K, E, dropped, wide = case
+    idx = make_idx(gen(T + K + E), T, K, E, dropped, wide)
+    p = ops.token_sort(idx.to(dev), E)
+    offsets, src, row, _ = sort_oracle(idx, E)
+    assert torch.equal(p.offsets.cpu(), offsets) and torch.equal(p.src.cpu(), src) and torch.equal(p.row.cpu(), row) and p.experts == E
+
+
+# tokens, top_k, experts, channels, row padding, share without an expert
+MOVES = [(1, 1, 2, 8, 0, 0.0), (7, 2, 3, 40, 8, 0.3), (33, 3, 5, 37, 0, 0.2), (16, 16, 20, 24, 4, 0.1), (5, 2, 4, 1, 0, 0.0), (130, 2, 4, 264, 0, 0.5), (4, 4, 4, 16, 0, 1.0), (3, 2, 4, 520, 0, 0.0)]
+
+
+def check_moves(ops, dtype, case, dev="cpu"):
+    import ctypes as C_
+
+    T, K, E, C, pad, dropped = case
+    g = gen(T * 7 + C)
+    idx = make_idx(g, T, K, E, dropped, False)
+    plan = ops.token_sort(idx.to(dev), E)
+    _, src, row, n = sort_oracle(idx, E)
+    tok = (src[:n] // K).long()
+    x = rows_of(g, T, C, dtype, pad, dev)
+    xs = ops.token_dispatch(x, plan)
+    assert xs.shape == (T * K, C) and torch.equal(xs[:n].cpu(), x.cpu()[tok])
+    # rows behind the last expert's, and the padding, stay as they were
+    buf = torch.full((T * K, C + 3), 7.0, dtype=dtype, device=dev)
+    es = buf.element_size()
+    rc = ops.lib.ymk_token_dispatch(C_.c_void_p(x.data_ptr()), (C + pad) * es if T > 1 else C * es, C * es, None, C_.c_void_p(buf.data_ptr()), (C + 3) * es, None,
+                                    C_.c_void_p(plan.row.data_ptr()), T, K, ops._stream())
+    assert rc == 0 and torch.equal(buf[:n, :C].cpu(), x.cpu()[tok]) and bool((buf[n:] == 7).all()) and bool((buf[:, C:] == 7).all())
+    ys = rows_of(g, T * K, C, dtype, pad, dev)
+    if n < T * K:
+        ys[n:] = float("nan")   # never read
+    w = torch.randn(T, K, generator=g)
+    w_ = torch.where(row >= 0, w, float("nan")).to(dev)   # nor is the weight of a pair without a row
+    kept = (row >= 0)[..., None]
+    part = torch.where(kept, ys.double().cpu()[row.clamp_min(0).long()], 0.0)
+    y64, mag = (part * w.double()[..., None]).sum(1), (part * w.double()[..., None]).abs().sum(1)
+    close(ops.token_combine(ys, plan, w_), y64, mag * (2 * K * U) + y64.abs() * half(dtype) + TINY[dtype], "combine")
+    close(ops.token_dispatch_backward(ys, plan), part.sum(1), part.abs().sum(1) * (2 * K * U) + part.sum(1).abs() * half(dtype) + TINY[dtype], "dispatch backward")
+    dy = rows_of(g, T, C, dtype, pad, dev)
+    dys, dw = ops.token_combine_backward(dy, ys, plan, w_)
+    d64 = w.reshape(-1)[src[:n].long()].double()[:, None] * dy.double().cpu()[tok]
+    close(dys[:n], d64, d64.abs() * (half(dtype) + U) + TINY[dtype], "dys")
+    t = part * dy.double().cpu()[:, None]
+    close(dw, t.sum(-1), t.abs().sum(-1) * ((C // 8 + 40) * U) + 1e-30, "dw")
+
+
+def check_dispatch_8bit(ops, dev="cpu"):
+    g = gen(3)
+    for C in (16, 40, 33):
+        x = torch.randint(0, 255, (9, C), generator=g, dtype=torch.uint8).view(torch.float8_e4m3fn)
+        scale = torch.rand(9, generator=g)
+        idx = make_idx(g, 9, 2, 4, 0.2, False)
+        xs, ss = ops.token_dispatch(x.to(dev), plan := ops.token_sort(idx.to(dev), 4), scale=scale.to(dev))
+        _, src, _, n = sort_oracle(idx, 4)
+        tok = (src[:n] // 2).long()
+        assert torch.equal(xs.view(torch.uint8)[:n].cpu(), x.view(torch.uint8)[tok]) and torch.equal(ss[:n].cpu(), scale[tok]) and plan.experts == 4
+
+
+# --------------------------------------------------------------------------------------------------------------- product
+# rows per expert, rows behind them, Cin, Cout, activation, row padding of x
+PRODUCTS = [([1], 0, 16, 16, None, 0), ([0, 3, 0, 5], 2, 64, 48, "silu", 16), ([130, 0, 1, 37], 3, 80, 144, "gelu", 0), ([5, 129], 0, 208, 16, "sigmoid", 0),
+            ([0, 0], 4, 32, 32, None, 0), ([64, 20], 0, 144, 272, None, 16)]
+
+
+def act64(v, act):
+    if act == "silu":
+        return v * torch.sigmoid(v)
+    if act == "gelu":
+        return 0.5 * v * (1 + torch.erf(v * 0.5**0.5))
+    return torch.sigmoid(v) if act == "sigmoid" else v
+
+
+def make_offsets(counts, start=0):
+    return torch.tensor([start] + (start + torch.tensor(counts).cumsum(0)).tolist(), dtype=torch.int32)
+
+
+def check_product(ops, dtype, case, dev="cpu", bias=True, start=0, out_dtype=None):
+    counts, behind, Cin, Cout, act, pad = case
+    g = gen(sum(counts) + Cin * 3 + Cout)
+    E, used = len(counts), sum(counts)
+    off = make_offsets(counts, start)
+    rows = start + used + behind
+    f8 = dtype == torch.float8_e4m3fn
+    b = 0.2 * torch.randn(E, Cout, generator=g)
+    live = torch.zeros(rows, dtype=torch.bool)
+    live[start:start + used] = True
+    if f8:
+        x32, w32 = torch.randn(rows, Cin, generator=g), torch.randn(E, Cout, Cin, generator=g)
+        xs, ws = x32.abs().amax(-1) / 448, w32.abs().amax(-1) / 448
+        x, w = (x32 / xs[:, None]).to(dtype), (w32 / ws[..., None]).to(dtype)
+        x.view(torch.uint8)[~live] = 0x7f   # NaN
+        x64, w64 = x.double() * xs.double()[:, None], w.double() * ws.double()[..., None]
+        buf = torch.full((rows, Cin + pad), 0x7f, dtype=torch.uint8)
+        buf[:, :Cin] = x.view(torch.uint8)
+        xd, wd = buf.view(dtype).to(dev)[:, :Cin], w.to(dev)
+        y = ops.expert_linear(xd, wd, off.to(dev), b.to(dev) if bias else None, act=act, x_scale=xs.to(dev), w_scale=ws.to(dev), out_dtype=out_dtype)
+        odt = out_dtype or torch.bfloat16
+    else:
+        xd = rows_of(g, rows, Cin, dtype, pad, dev)
+        xd[~live.to(dev)] = float("nan")
+        w = (torch.randn(E, Cout, Cin, generator=g) * Cin**-0.5).to(dtype)
+        x64, w64, wd, odt = xd.double().cpu(), w.double(), w.to(dev), dtype
+        y = ops.expert_linear(xd, wd, off.to(dev), b.to(dev) if bias else None, act=act)
+    assert y.dtype == odt and y.shape == (rows, Cout)
+    for e, n in enumerate(counts):
+        s = slice(int(off[e]), int(off[e]) + n)
+        v = x64[s] @ w64[e].t()
+        mag = x64[s].abs() @ w64[e].abs().t() + 1
+        if bias:
+            v = v + b[e].double()
+        want = act64(v, act)
+        if f8 and len(v):
+            # The 8-bit matrix instruction adds 16 products at the largest one's exponent and drops what lies below 2^-13 of it (1 - 1 + 2^-12 gives
+            # 2^-12, 1 - 1 + 2^-14 gives 0, in 16 places of K; in different 16 both survive).  So a product loses less than 2^-12 of the group's
+            # largest, and a 64-deep instruction less than 4 * 15 * 2^-12 of the largest of its 64.
+            p = (x64[s][:, None] * w64[e][None]).abs()
+            p = torch.nn.functional.pad(p, (0, -Cin % 64)).unflatten(-1, (-1, 64)).amax(-1).sum(-1)
+            mag = mag + p * (60 * 2.0**-12) / (U * (Cin + 8))
+        # (Cin + 8) additions and scalings before the activation, whose slope is at most 1.13 and which adds a few roundings of its own
+        close(y[s], want, mag * (1.13 * (Cin + 8) + 8) * U + want.abs() * half(odt) + TINY[odt], f"expert {e}")
+
+
+def check_product_exact(ops, case, dev="cpu"):
+    """8-bit codes whose products span fewer bits than the instruction keeps, and scales that are powers of two: every sum is exact, so is the output."""
+    counts, behind, Cin, Cout, _, _ = case
+    g = gen(Cin + Cout)
+    E, rows = len(counts), sum(counts) + behind
+    pick = lambda *s: (torch.randint(8, 16, s, generator=g) * torch.tensor([0.125, 0.25, -0.25])[torch.randint(0, 3, s, generator=g)]).to(torch.float8_e4m3fn)   # noqa: E731
+    x, w = pick(rows, Cin), pick(E, Cout, Cin)
+    xs, ws = 2.0 ** torch.randint(-3, 3, (rows,), generator=g).float(), 2.0 ** torch.randint(-3, 3, (E, Cout), generator=g).float()
+    off = make_offsets(counts)
+    y = ops.expert_linear(x.to(dev), w.to(dev), off.to(dev), x_scale=xs.to(dev), w_scale=ws.to(dev), out_dtype=torch.float32).cpu()
+    for e, n in enumerate(counts):
+        s = slice(int(off[e]), int(off[e]) + n)
+        assert torch.equal(y[s].double(), (x[s].double() @ w[e].double().t()) * xs[s].double()[:, None] * ws[e].double()), e
+
+
+def check_product_gradient(ops, dtype, case, dev="cpu", dw_dtype=None):
+    counts, behind, Cin, Cout, _, pad = case
+    g = gen(sum(counts) + Cin + Cout * 5)
+    E, used = len(counts), sum(counts)
+    off = make_offsets(counts)
+    rows = used + behind
+    x, dy = rows_of(g, rows, Cin, dtype, pad, dev), rows_of(g, rows, Cout, dtype, pad, dev)
+    if behind:
+        x[used:], dy[used:] = float("nan"), float("nan")
+    w = (torch.randn(E, Cout, Cin, generator=g) * Cin**-0.5).to(dtype).to(dev)
+    dx, dw, db = ops.expert_linear_backward(dy, x, w, off.to(dev), dw_dtype=dw_dtype)
+    odt = dw_dtype or dtype
+    assert dx.dtype == dtype and dw.dtype == odt and db.dtype == torch.float32
+    x64, d64, w64 = x.double().cpu(), dy.double().cpu(), w.double().cpu()
+    for e, n in enumerate(counts):
+        s = slice(int(off[e]), int(off[e]) + n)
+        want = d64[s] @ w64[e]
+        close(dx[s], want, (d64[s].abs() @ w64[e].abs()) * ((Cout + 8) * U) + want.abs() * half(dtype) + TINY[dtype], f"dx {e}")
+        want = d64[s].t() @ x64[s]
+        close(dw[e], want, (d64[s].abs().t() @ x64[s].abs()) * ((n + 8) * U) + want.abs() * half(odt) + TINY[odt], f"dw {e}")
+        close(db[e], d64[s].sum(0), d64[s].abs().sum(0) * ((n + 8) * U) + 1e-30, f"db {e}")
+    only = ops.expert_linear_backward(dy, x, w, off.to(dev), need_dx=False, need_db=False, dw_dtype=dw_dtype)
+    assert only[0] is None and only[2] is None and torch.equal(only[1], dw)
+
+
+# -------------------------------------------------------------------------------------------- as they are used together
+def expert_block(ops, x, res, p, K, dtype):
+    """A pre-norm expert layer of a serving program: residual sum, norm, routing, two products with an activation, and back."""
+    y, h, _ = ops.rms_norm(x, p["norm"], residual=res)
+    score = (y.float() @ p["router"]).softmax(-1)
+    gate, idx = score.topk(K, dim=-1)
+    plan = ops.token_sort(idx, p["w1"].shape[0])
+    a = ops.expert_linear(ops.token_dispatch(y, plan), p["w1"], plan.offsets, p["b1"], act="gelu")
+    return ops.token_combine(ops.expert_linear(a, p["w2"], plan.offsets, p["b2"]), plan, gate.contiguous()), h, plan, gate, y, a
+
+
+def block_params(g, C, H, E, dtype, dev):
+    r = lambda *s: torch.randn(*s, generator=g)   # noqa: E731
+    return {"norm": (1 + 0.1 * r(C)).to(dev), "router": (r(C, E) * C**-0.5).to(dev), "w1": (r(E, H, C) * C**-0.5).to(dtype).to(dev), "b1": (0.1 * r(E, H)).to(dev),
+            "w2": (r(E, C, H) * H**-0.5).to(dtype).to(dev), "b2": (0.1 * r(E, C)).to(dev)}
+
+
+def check_block(ops, dtype, dev="cpu", T=23, C=64, H=128, E=5, K=2):
+    g = gen(T + C)
+    x, res, p = rows_of(g, T, C, dtype, 0, dev), rows_of(g, T, C, dtype, 0, dev), block_params(g, C, H, E, dtype, dev)
+    out, h, plan, gate, y, a = expert_block(ops, x, res, p, K, dtype)
+    d = {k: v.double().cpu() for k, v in p.items()}
+    y64 = y.double().cpu()   # the router's choice is taken as made: it depends on the norm's rounding
+    row, src = plan.row.cpu().long(), plan.src.cpu().long()
+    off = plan.offsets.cpu()
+    e = torch.bucketize(row.reshape(-1), off[1:].long(), right=True).reshape(row.shape)
+    want = torch.zeros(T, C, dtype=torch.float64)
+    mag = torch.zeros(T, C, dtype=torch.float64)
+    for k in range(K):
+        for t in range(T):
+            a64 = act64(d["w1"][e[t, k]] @ y64[t] + d["b1"][e[t, k]], "gelu")
+            z = d["w2"][e[t, k]] @ a64 + d["b2"][e[t, k]]
+            want[t] += gate[t, k].double().cpu() * z
+            # the hidden row is rounded once, its products add up; the expert's answer is rounded once
+            mag[t] += gate[t, k].double().cpu() * (d["w2"][e[t, k]].abs() @ a64.abs() + z.abs())
+    close(out, want, mag * (half(dtype) * 1.2 + (C + H + 32) * U) + want.abs() * half(dtype) + TINY[dtype], "block")
+    assert torch.equal(h, (x.float() + res.float()).to(dtype)) and int(off[-1]) == T * K and torch.equal(src.sort().values, torch.arange(T * K))
+
+
+def check_block_gradient(ops, dev="cpu", T=11, C=32, H=48, E=3, K=2):
+    """The gradients chained by hand, in fp32, against autograd of the same block in 64 bits."""
+    g = gen(77)
+    x, res, p = rows_of(g, T, C, torch.float32, 0, dev), rows_of(g, T, C, torch.float32, 0, dev), block_params(g, C, H, E, torch.float32, dev)
+    y, h, rstd = ops.rms_norm(x, p["norm"], residual=res)
+    gate = torch.rand(T, K, generator=g).to(dev)
+    idx = torch.stack([torch.randperm(E, generator=g)[:K] for _ in range(T)]).to(dev)
+    plan = ops.token_sort(idx, E)
+    xs = ops.token_dispatch(y, plan)
+    a1 = ops.expert_linear(xs, p["w1"], plan.offsets, p["b1"])
+    a = a1 * torch.sigmoid(a1)
+    z = ops.expert_linear(a, p["w2"], plan.offsets, p["b2"])
+    out = ops.token_combine(z, plan, gate)
+    dout = torch.randn(T, C, generator=g).to(dev)
+    dz, dgate = ops.token_combine_backward(dout, z, plan, gate)
+    da, dw2, db2 = ops.expert_linear_backward(dz, a, p["w2"], plan.offsets)
+    s = torch.sigmoid(a1)
+    da1 = da * (s * (1 + a1 * (1 - s)))
+    dxs, dw1, db1 = ops.expert_linear_backward(da1, xs, p["w1"], plan.offsets)
+    dx, dnorm = ops.rms_norm_backward(ops.token_dispatch_backward(dxs, plan), h, p["norm"], rstd, dres=dout)   # out + h leave the block
+    q = {k: v.double().cpu().requires_grad_(True) for k, v in p.items() if k != "router"}
+    x64, gate64 = x.double().cpu().requires_grad_(True), gate.double().cpu().requires_grad_(True)
+    h64 = x64 + res.double().cpu()
+    y64 = h64 * (h64.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * q["norm"]
+    ref = torch.zeros(T, C, dtype=torch.float64)
+    for k in range(K):
+        e = idx[:, k].cpu()
+        v = torch.nn.functional.silu((q["w1"][e] @ y64[..., None])[..., 0] + q["b1"][e])
+        ref = ref + gate64[:, k, None] * ((q["w2"][e] @ v[..., None])[..., 0] + q["b2"][e])
+    ((ref + h64) * dout.double().cpu()).sum().backward()
+    # a chain of five fp32 operators, each within (its length + 40) u of its terms' magnitudes, whose sums exceed the results by some tens here
+    for got, want, what in ((out, ref.detach(), "out"), (dx, x64.grad, "dx"), (dnorm, q["norm"].grad, "dnorm"), (dgate, gate64.grad, "dgate"), (dw1, q["w1"].grad, "dw1"),
+                            (db1, q["b1"].grad, "db1"), (dw2, q["w2"].grad, "dw2"), (db2, q["b2"].grad, "db2")):
+        close(got, want, torch.full_like(want, 5 * 128 * 40 * U * float(want.abs().max())), what)

@@ -10,7 +10,7 @@ import ctypes as C
 import os
 from pathlib import Path
 
-__all__ = ["lib", "load", "YmkLibraryError", "ConvDesc", "check", "LIB_PATH", "SYMBOLS", "SYMBOLS_MIXTURE", "SYMBOLS_NEXT"]
+__all__ = ["lib", "load", "YmkLibraryError", "ConvDesc", "check", "LIB_PATH", "SYMBOLS", "SYMBOLS_MIXTURE", "SYMBOLS_NEXT", "SYMBOLS_TOKENS"]
 
 LIB_PATH = Path(__file__).resolve().parent / "libymk.so"
 LIB_F16_PATH = Path(__file__).resolve().parent / "libymk_f16.so"   # the same sources / ABI, 16-bit element format = IEEE binary16
@@ -140,6 +140,23 @@ SYMBOLS_NEXT = {
     "ymk_match_predictions": (C.c_int, [_vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _f32, _vp, _vp, _sz, _vp]),
     "ymk_letterbox_preprocess": (C.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
+# include/ymk_tokens.h: norms with an 8-bit output, tokens by expert, the experts' product, and their gradients
+SYMBOLS_TOKENS = {
+    "ymk_rms_norm": (C.c_int, [_i32, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i64, _i32, _vp, _f32, _vp]),
+    "ymk_rms_norm_quant": (C.c_int, [_i32, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i64, _i32, _vp, _f32, _vp]),
+    "ymk_rms_norm_backward_workspace_bytes": (_sz, [_i64, _i32]),
+    "ymk_rms_norm_backward": (C.c_int, [_i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _i64, _i32, _vp, _sz, _vp]),
+    "ymk_token_sort_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "ymk_token_sort": (C.c_int, [_vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ymk_token_dispatch": (C.c_int, [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _vp]),
+    "ymk_token_combine": (C.c_int, [_i32, _vp, _i32, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp]),
+    "ymk_token_combine_backward": (C.c_int, [_i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _i32, _i32, _vp]),
+    "ymk_expert_linear": (C.c_int, [_i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "ymk_expert_linear_dx": (C.c_int, [_i32, _vp, _i32, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _vp]),
+    "ymk_expert_linear_dw": (C.c_int, [_i32, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
+}
+YMK_E4M3 = 2
+NORM_MAX_C, TOKEN_MAX_E, TOKEN_MAX_K = 16384, 256, 16
 ACT_SIGMOID, ACT_GELU = 2, 3
 ELT_MUL, ELT_SIGMOID_MUL, ELT_LERP, ELT_CLAMP_ADD = 0, 1, 2, 3
 
@@ -183,7 +200,7 @@ def load(path: os.PathLike | None = None) -> C.CDLL:
         except AttributeError as e:
             raise YmkLibraryError(f"{p} does not export {name}; rebuild libymk") from e
         fn.restype, fn.argtypes = res, args
-    for name, (res, args) in {**SYMBOLS_MIXTURE, **SYMBOLS_NEXT}.items():
+    for name, (res, args) in {**SYMBOLS_MIXTURE, **SYMBOLS_NEXT, **SYMBOLS_TOKENS}.items():
         try:
             fn = getattr(h, name)
         except AttributeError as e:

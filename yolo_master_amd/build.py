@@ -21,11 +21,15 @@ LIB = HERE / "libymk.so"
 VARIANTS = {"bf16": (OBJ, LIB, []), "f16": (CSRC / "_obj_f16", HERE / "libymk_f16.so", ["-DYMK_H16_F16"])}
 ARCH = "gfx950"
 # files whose arithmetic must not be contracted into FMAs (bit-exact NMS / decode)
+# The compiler's own packed fp32 instructions stay out of the kernels (some of their forms are not reliable on this hardware)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 NO_CONTRACT = {"nms.hip", "elementwise.hip", "post.hip", "preproc.hip"}
+TOKEN_SOURCES = ["rmsnorm.hip", "tokens.hip", "expert.hip"]   # norms, tokens by expert, the experts' product (include/ymk_tokens.h)
 SOURCES = ["capi.hip", "conv.hip", "dwconv.hip", "mlp.hip", "stem2.hip", "c3k2f.hip", "detcls.hip", "esmoe.hip", "attn.hip", "elementwise.hip", "nms.hip",
            "mixture.hip", "mixattn.hip",   # config-5 rows, first implementation (include/ymk_mixture.h)
+           *TOKEN_SOURCES,
            "conv_glds.hip", "post.hip", "preproc.hip"]   # LDS-DMA tiled convolution core, box rescaling / validation matching, letterbox (include/ymk_next.h)
-HEADERS = ["ymk_common.h", "igemm.h", "glds.h", "../../include/ymk.h", "../../include/ymk_mixture.h", "../../include/ymk_next.h"]
+HEADERS = ["ymk_common.h", "igemm.h", "glds.h", "../../include/ymk.h", "../../include/ymk_mixture.h", "../../include/ymk_next.h", "../../include/ymk_tokens.h"]
 
 
 def _hipcc() -> str:
@@ -48,7 +52,7 @@ def source_hash() -> str:
 
 
 def _compile_cmd(hipcc: str, src: str, obj: Path, defs: list) -> list:
-    cmd = [hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", *defs, "-c", str(CSRC / src), "-o", str(obj)]
+    cmd = [hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", *defs, *(NO_PACKED_FP32 if src in TOKEN_SOURCES else []), "-c", str(CSRC / src), "-o", str(obj)]
     if src in NO_CONTRACT:
         cmd.insert(4, "-ffp-contract=off")
     if src in ("post.hip", "preproc.hip"):   # bit-exact box rescaling divides by the gain: IEEE division (hipcc's default, stated explicitly)

@@ -13,6 +13,7 @@ import os
 import torch
 
 import threading
+from typing import NamedTuple
 
 from . import _lib
 from ._lib import ConvDesc, check
@@ -1184,3 +1185,327 @@ def tokens_to_rows(x, y, a_off: int, row_off: int = 0):
     check(lib.ymk_tokens_to_rows(DT[x.dtype], _p(x), ldx, _p(y), B, H * W, Cc, a_off, y.shape[2], row_off, y.shape[1], _stream()),
           "tokens_to_rows")
     return y
+
+
+# ----------------------------------------------------------------------------- tokens (include/ymk_tokens.h)
+# Rows instead of maps: [..., C] tensors whose last dim is dense and whose leading dims are one run of rows (any row stride >= C).  All operands of a
+# call live on the current device; outputs are new tensors of the current stream.  Gradients are calls of their own, for a training program's
+# autograd functions: these wrappers keep nothing between calls.
+E4M3 = torch.float8_e4m3fn
+_ROW_DT = {**DT, E4M3: _lib.YMK_E4M3}
+_ROW_ACT = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "sigmoid": _lib.ACT_SIGMOID}
+
+
+def _rows(t: torch.Tensor, what: str):
+    """(rows, C, ld) of a row view."""
+    if t.dim() == 2:
+        M, Cc = t.shape
+        ld = t.stride(0)
+    elif t.dim() > 2:
+        Cc, M, ld = t.shape[-1], 1, 0
+        for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if n == 1:
+                continue
+            if M == 1:
+                ld = s
+            elif s != M * ld:
+                raise ValueError(f"{what}: the rows of the view are not evenly spaced")
+            M *= n
+    else:
+        raise ValueError(f"{what}: expected [..., C], got {tuple(t.shape)}")
+    if Cc > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: the last dim must be dense")
+    if M <= 1:
+        return M, Cc, Cc
+    if ld < Cc:
+        raise ValueError(f"{what}: rows overlap (row stride {ld} < {Cc})")
+    return M, Cc, ld
+
+
+def _here(what: str, first: torch.Tensor, *others) -> None:
+    """All operands on one GPU, and that the current one (the call goes to its current stream)."""
+    require_gpu(first, what)
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: operands on {dev} and {t.device}")
+    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: operands on {dev}, current device cuda:{torch.cuda.current_device()}")
+
+
+def _fp32_vec(t, shape, what: str, name: str) -> None:
+    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} is a contiguous fp32 {list(shape)} tensor, got {t.dtype} {list(t.shape)}")
+
+
+def _like(t, x, what: str, name: str):
+    """t's row stride; t is a view of x's shape and dtype."""
+    if t.dtype != x.dtype or t.shape != x.shape:
+        raise ValueError(f"{what}: {name} is {t.dtype} {list(t.shape)}, expected {x.dtype} {list(x.shape)}")
+    return _rows(t, what)[2]
+
+
+def _norm_args(what, x, weight, residual, residual_out):
+    if x.dtype not in DT:
+        raise ValueError(f"{what}: dtype {x.dtype}")
+    _here(what, x, weight, residual, residual_out)
+    M, Cc, ldx = _rows(x, what)
+    if not 1 <= Cc <= _lib.NORM_MAX_C:
+        raise ValueError(f"{what}: {Cc} channels (1 .. {_lib.NORM_MAX_C})")
+    _fp32_vec(weight, (Cc,), what, "weight")
+    use_format(x.dtype)
+    if residual is None:
+        if residual_out is not None:
+            raise ValueError(f"{what}: residual_out without a residual")
+        return M, Cc, ldx, 0, x, 0
+    ldr = _like(residual, x, what, "residual")
+    if residual_out is None:
+        return M, Cc, ldx, ldr, torch.empty(x.shape, dtype=x.dtype, device=x.device), Cc
+    ldh = _like(residual_out, x, what, "residual_out")
+    for t, ld in ((x, ldx), (residual, ldr)):   # in place is fine, row by row; a shifted view is not
+        a, b = t.data_ptr(), residual_out.data_ptr()
+        span = ((M - 1) * max(ld, ldh) + Cc) * x.element_size()
+        if M and not (a == b and (ld == ldh or M == 1)) and abs(a - b) < span:
+            raise ValueError(f"{what}: residual_out overlaps an input without being it")
+    return M, Cc, ldx, ldr, residual_out, ldh
+
+
+@_timed("rms_norm")
+def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
+    """h = x + residual (rounded to x's dtype; h is x without a residual), y = h / sqrt(mean(h^2) + eps) * weight.  Returns (y, h, rstd); rstd
+    fp32, one a row, is what rms_norm_backward takes.  residual_out: where h goes (x or residual themselves, or a tensor apart from them)."""
+    M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm", x, weight, residual, residual_out)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    check(lib.ymk_rms_norm(DT[x.dtype], _p(x), ldx, _p(residual), ldr, _p(h) if residual is not None else None, ldh, _p(y), Cc, _p(rstd), M, Cc, _p(weight),
+                           float(eps), _stream()), "rms_norm")
+    return y, h, rstd
+
+
+@_timed("rms_norm")
+def rms_norm_quant(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
+    """The same norm with an 8-bit output: (q, scale, h), q e4m3 of x's shape and scale fp32 per row with y = q * scale, max |q| = 448
+    (an all-zero row: scale 1; a row with a NaN or an infinity: all NaN)."""
+    M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm_quant", x, weight, residual, residual_out)
+    q = torch.empty(x.shape, dtype=E4M3, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    check(lib.ymk_rms_norm_quant(DT[x.dtype], _p(x), ldx, _p(residual), ldr, _p(h) if residual is not None else None, ldh, _p(q), Cc, _p(scale), M, Cc,
+                                 _p(weight), float(eps), _stream()), "rms_norm_quant")
+    return q, scale, h
+
+
+@_timed("rms_norm")
+def rms_norm_backward(dy, h, weight, rstd, dres=None, need_dweight: bool = True):
+    """Gradient of rms_norm: (dx, dweight) from dy and the h, rstd it returned; dres is the gradient that reaches h by its other use (the residual
+    stream).  dx is the gradient of x and of residual alike; dweight fp32 (None unless wanted)."""
+    what = "rms_norm_backward"
+    if h.dtype not in DT:
+        raise ValueError(f"{what}: dtype {h.dtype}")
+    _here(what, h, dy, weight, rstd, dres)
+    M, Cc, ldh = _rows(h, what)
+    if not 1 <= Cc <= _lib.NORM_MAX_C:
+        raise ValueError(f"{what}: {Cc} channels (1 .. {_lib.NORM_MAX_C})")
+    _fp32_vec(weight, (Cc,), what, "weight")
+    _fp32_vec(rstd, h.shape[:-1], what, "rstd")
+    lddy = _like(dy, h, what, "dy")
+    lddr = _like(dres, h, what, "dres") if dres is not None else 0
+    use_format(h.dtype)
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dweight = ws = None
+    nbytes = 0
+    if need_dweight:
+        dweight = torch.empty((Cc,), dtype=torch.float32, device=h.device)
+        nbytes = lib.ymk_rms_norm_backward_workspace_bytes(M, Cc)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=h.device)
+    check(lib.ymk_rms_norm_backward(DT[h.dtype], _p(dy), lddy, _p(h), ldh, _p(rstd), _p(weight), _p(dres), lddr, _p(dx), Cc, _p(dweight), M, Cc, _p(ws),
+                                    nbytes, _stream()), what)
+    return dx, dweight
+
+
+class TokenPlan(NamedTuple):
+    """Where every (token, choice) pair goes: rows offsets[e] .. offsets[e + 1] are expert e's; src[row] = token * top_k + choice, -1 behind the last
+    row; row[token][choice] = its row, -1 for a pair without an expert.  All int32 on the device; the host never learns the counts."""
+
+    offsets: torch.Tensor
+    src: torch.Tensor
+    row: torch.Tensor
+    experts: int
+
+
+@_timed("token_sort")
+def token_sort(idx, experts: int) -> TokenPlan:
+    """Stable sort of the pairs idx [tokens, top_k] (int32 or int64; values outside [0, experts) have no expert) by expert."""
+    if idx.dim() != 2 or idx.dtype not in (torch.int32, torch.int64) or not idx.is_contiguous():
+        raise ValueError("token_sort: idx is a contiguous int32 or int64 [tokens, top_k] tensor")
+    _here("token_sort", idx)
+    T, K = idx.shape
+    if not 1 <= K <= _lib.TOKEN_MAX_K or not 1 <= experts <= _lib.TOKEN_MAX_E or T * K >= 1 << 30:
+        raise ValueError(f"token_sort: top_k {K} (1 .. {_lib.TOKEN_MAX_K}), {experts} experts (1 .. {_lib.TOKEN_MAX_E}), {T} tokens")
+    dev = idx.device
+    offsets = torch.empty((experts + 1,), dtype=torch.int32, device=dev)
+    src = torch.empty((T * K,), dtype=torch.int32, device=dev)
+    row = torch.empty((T, K), dtype=torch.int32, device=dev)
+    nbytes = lib.ymk_token_sort_workspace_bytes(T, K, experts)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+    check(lib.ymk_token_sort(_p(idx), idx.element_size(), T, K, experts, _p(offsets), _p(src), _p(row), _p(ws), nbytes, _stream()), "token_sort")
+    return TokenPlan(offsets, src, row, experts)
+
+
+def _planned(what, plan, t, rows=None):
+    """(tokens, top_k) of the plan; t has a row for every token, or (rows) for every pair."""
+    T, K = plan.row.shape
+    M, Cc, ld = _rows(t, what)
+    if M != (T * K if rows else T) or Cc < 1:
+        raise ValueError(f"{what}: {M} rows for a plan of {T} tokens by {K}")
+    return T, K, Cc, ld
+
+
+@_timed("token_move")
+def token_dispatch(x, plan: TokenPlan, scale=None):
+    """xs[plan.row[t][k]] = x[t], any element type; with scale (fp32 [tokens], of an 8-bit x) -> (xs, xs_scale).  Rows behind the last expert's are
+    not written."""
+    _here("token_dispatch", x, plan.row, scale)
+    T, K, Cc, ldx = _planned("token_dispatch", plan, x)
+    es = x.element_size()
+    xs = torch.empty((T * K, Cc), dtype=x.dtype, device=x.device)
+    xs_scale = None
+    if scale is not None:
+        if scale.numel() != T or scale.dtype != torch.float32 or not scale.is_contiguous():
+            raise ValueError(f"token_dispatch: scale is contiguous fp32, one a token ({T})")
+        xs_scale = torch.empty((T * K,), dtype=torch.float32, device=x.device)
+    check(lib.ymk_token_dispatch(_p(x), ldx * es, Cc * es, _p(scale), _p(xs), Cc * es, _p(xs_scale), _p(plan.row), T, K, _stream()), "token_dispatch")
+    return xs if scale is None else (xs, xs_scale)
+
+
+def _combine(what, ys, plan, w):
+    if ys.dtype not in DT:
+        raise ValueError(f"{what}: dtype {ys.dtype}")
+    _here(what, ys, plan.row, w)
+    T, K, Cc, ldys = _planned(what, plan, ys, rows=True)
+    if w is not None:
+        _fp32_vec(w, (T, K), what, "w")
+    use_format(ys.dtype)
+    y = torch.empty((T, Cc), dtype=ys.dtype, device=ys.device)
+    check(lib.ymk_token_combine(DT[ys.dtype], _p(ys), ldys, _p(plan.row), _p(w), _p(y), Cc, T, K, Cc, _stream()), what)
+    return y
+
+
+@_timed("token_move")
+def token_combine(ys, plan: TokenPlan, w):
+    """y[t] = sum over k of w[t][k] * ys[plan.row[t][k]] (fp32, in the order of k); w fp32 [tokens, top_k].  A token without any row gets zeros."""
+    if w is None:
+        raise ValueError("token_combine: w is required")
+    return _combine("token_combine", ys, plan, w)
+
+
+@_timed("token_move")
+def token_dispatch_backward(dxs, plan: TokenPlan):
+    """Gradient of token_dispatch: dx[t] = the sum of dxs over the token's rows."""
+    return _combine("token_dispatch_backward", dxs, plan, None)
+
+
+@_timed("token_move")
+def token_combine_backward(dy, ys, plan: TokenPlan, w):
+    """Gradient of token_combine: (dys, dw), dys[plan.row[t][k]] = w[t][k] * dy[t], dw[t][k] = <dy[t], ys[plan.row[t][k]]> in fp32 (0 for a pair
+    without a row).  Rows of dys behind the last expert's are not written."""
+    what = "token_combine_backward"
+    if ys.dtype not in DT or dy.dtype != ys.dtype:
+        raise ValueError(f"{what}: dtypes {dy.dtype}, {ys.dtype}")
+    _here(what, ys, dy, plan.row, w)
+    T, K, Cc, ldys = _planned(what, plan, ys, rows=True)
+    _, _, Cd, lddy = _planned(what, plan, dy)
+    if Cd != Cc:
+        raise ValueError(f"{what}: dy has {Cd} channels, ys {Cc}")
+    _fp32_vec(w, (T, K), what, "w")
+    use_format(ys.dtype)
+    dys = torch.empty((T * K, Cc), dtype=ys.dtype, device=ys.device)
+    dw = torch.empty((T, K), dtype=torch.float32, device=ys.device)
+    check(lib.ymk_token_combine_backward(DT[ys.dtype], _p(dy), lddy, _p(ys), ldys, _p(plan.row), _p(w), _p(dys), Cc, _p(dw), T, K, Cc, _stream()), what)
+    return dys, dw
+
+
+def _expert_args(what, x, w, offsets):
+    if x.dtype not in _ROW_DT or w.dtype != x.dtype:
+        raise ValueError(f"{what}: rows {x.dtype}, weights {w.dtype}")
+    if w.dim() != 3 or not w.is_contiguous() or 0 in w.shape:
+        raise ValueError(f"{what}: w is a contiguous [experts, Cout, Cin] tensor, got {list(w.shape)}")
+    E, Cout, Cin = w.shape
+    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (E + 1,) or not offsets.is_contiguous():
+        raise ValueError(f"{what}: offsets is a contiguous int32 [{E + 1}] tensor")
+    if E > _lib.TOKEN_MAX_E:
+        raise ValueError(f"{what}: {E} experts (at most {_lib.TOKEN_MAX_E})")
+    if x.dtype in H16:
+        use_format(x.dtype)
+    return E, Cout, Cin
+
+
+def _expert_rows(what, t, Cc):
+    M, c, ld = _rows(t, what)
+    if c != Cc:
+        raise ValueError(f"{what}: rows of {c} channels, expected {Cc}")
+    if t.data_ptr() % 16 or ld * t.element_size() % 16 or Cc * t.element_size() % 16:
+        raise ValueError(f"{what}: rows of {Cc} x {t.dtype} at a stride of {ld} are not 16-byte aligned")
+    return M, ld
+
+
+@_timed("expert_linear", flops=lambda x, w, *a, **k: 2 * x.numel() * w.shape[1])
+def expert_linear(x, w, offsets, bias=None, act=None, x_scale=None, w_scale=None, out_dtype=None):
+    """y[r] = act(x[r] @ w[e].T + bias[e]) for the rows offsets[e] <= r < offsets[e + 1] (TokenPlan.offsets); rows outside every expert are not written.
+    x [rows, Cin], w [experts, Cout, Cin] of one dtype (fp32, 16-bit, or e4m3 with x_scale fp32 [rows] and w_scale fp32 [experts, Cout]), bias fp32
+    [experts, Cout], act None | "silu" | "gelu" | "sigmoid".  The output has x's dtype; e4m3 rows give out_dtype (bfloat16 unless said)."""
+    what = "expert_linear"
+    E, Cout, Cin = _expert_args(what, x, w, offsets)
+    _here(what, x, w, offsets, bias, x_scale, w_scale)
+    M, ldx = _expert_rows(what, x, Cin)
+    odt = x.dtype
+    if x.dtype == E4M3:
+        odt = out_dtype or torch.bfloat16
+        if odt not in DT:
+            raise ValueError(f"{what}: out_dtype {odt}")
+        if x_scale is None or w_scale is None:
+            raise ValueError(f"{what}: e4m3 operands need x_scale and w_scale")
+        _fp32_vec(x_scale, (M,), what, "x_scale")
+        _fp32_vec(w_scale, (E, Cout), what, "w_scale")
+        if odt in H16:
+            use_format(odt)
+    elif x_scale is not None or w_scale is not None or out_dtype not in (None, x.dtype):
+        raise ValueError(f"{what}: scales and another out_dtype belong to e4m3 operands")
+    if Cout % (8 if odt != torch.float32 or x.dtype == E4M3 else 4) or w.data_ptr() % 16:
+        raise ValueError(f"{what}: {Cout} output channels do not fill 16-byte pieces, or w is not 16-byte aligned")
+    if bias is not None:
+        _fp32_vec(bias, (E, Cout), what, "bias")
+    if act not in _ROW_ACT:
+        raise ValueError(f"{what}: act {act!r}")
+    y = torch.empty((M, Cout), dtype=odt, device=x.device)
+    check(lib.ymk_expert_linear(_ROW_DT[x.dtype], DT[odt], _p(x), ldx, _p(x_scale), _p(w), _p(w_scale), _p(bias), _p(offsets), _p(y), Cout, M, E, Cin, Cout,
+                                _ROW_ACT[act], _stream()), what)
+    return y
+
+
+@_timed("expert_linear", flops=lambda dy, x, w, *a, **k: 4 * x.numel() * w.shape[1])
+def expert_linear_backward(dy, x, w, offsets, need_dx: bool = True, need_dw: bool = True, need_db: bool = True, dw_dtype=None):
+    """Gradient of expert_linear without activation: (dx, dw, db); None for what is not wanted (db comes with dw).  dx[r] = dy[r] @ w[e]; dw[e] = dy_e.T @
+    x_e in w's dtype or dw_dtype=torch.float32; db fp32.  An expert without rows gets zeros; rows of dx outside every expert are not written."""
+    what = "expert_linear_backward"
+    E, Cout, Cin = _expert_args(what, x, w, offsets)
+    if x.dtype not in DT or dy.dtype != x.dtype:
+        raise ValueError(f"{what}: rows {x.dtype}, dy {dy.dtype}")
+    if dw_dtype not in (None, x.dtype, torch.float32):
+        raise ValueError(f"{what}: dw_dtype {dw_dtype}")
+    if need_db and not need_dw:
+        raise ValueError(f"{what}: db comes with dw")
+    _here(what, x, dy, w, offsets)
+    M, ldx = _expert_rows(what, x, Cin)
+    Md, lddy = _expert_rows(what, dy, Cout)
+    if Md != M or w.data_ptr() % 16:
+        raise ValueError(f"{what}: {M} rows of x, {Md} of dy, or w is not 16-byte aligned")
+    dx = dw = db = None
+    if need_dx:
+        dx = torch.empty((M, Cin), dtype=x.dtype, device=x.device)
+        check(lib.ymk_expert_linear_dx(DT[x.dtype], _p(dy), lddy, _p(w), _p(offsets), _p(dx), Cin, M, E, Cin, Cout, _stream()), "expert_linear_dx")
+    if need_dw:
+        dw = torch.empty((E, Cout, Cin), dtype=dw_dtype or x.dtype, device=x.device)
+        db = torch.empty((E, Cout), dtype=torch.float32, device=x.device) if need_db else None
+        check(lib.ymk_expert_linear_dw(DT[x.dtype], DT[dw.dtype], _p(dy), lddy, _p(x), ldx, _p(offsets), _p(dw), _p(db), M, E, Cin, Cout, _stream()),
+              "expert_linear_dw")
+    return dx, dw, db
