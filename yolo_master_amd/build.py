@@ -21,7 +21,8 @@ LIB = HERE / "libymk.so"
 VARIANTS = {"bf16": (OBJ, LIB, []), "f16": (CSRC / "_obj_f16", HERE / "libymk_f16.so", ["-DYMK_H16_F16"])}
 ARCH = "gfx950"
 # files whose arithmetic must not be contracted into FMAs (bit-exact NMS / decode)
-# The compiler's own packed fp32 instructions stay out of the kernels (some of their forms are not reliable on this hardware)
+# Packed fp32 instructions stay out of all kernels (some of their forms have given wrong results on this hardware): fp32 pair arithmetic in the sources
+# (csrc/dwconv.hip) compiles to two instructions.  The detector's step takes the same time either way (4.87 ms, two runs of each differ by 1.5 %).
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 NO_CONTRACT = {"nms.hip", "elementwise.hip", "post.hip", "preproc.hip"}
 TOKEN_SOURCES = ["rmsnorm.hip", "tokens.hip", "expert.hip"]   # norms, tokens by expert, the experts' product (include/ymk_tokens.h)
@@ -40,19 +41,19 @@ def _hipcc() -> str:
 
 
 def source_hash() -> str:
-    """sha256 (16 hex digits) over the kernel sources and shared headers: committed rocprofv3 summaries carry it, so that a
+    """sha256 (16 hex digits) over the detector's kernel sources and shared headers: committed rocprofv3 summaries carry it, so that a
     profile is only ever quoted for the kernels it was collected on (bench.py `roofline.traffic`, `families[].sq`)."""
     import hashlib
 
     h = hashlib.sha256()
-    for f in sorted(SOURCES) + ["ymk_common.h", "igemm.h", "glds.h"]:
+    for f in sorted(set(SOURCES) - set(TOKEN_SOURCES)) + ["ymk_common.h", "igemm.h", "glds.h"]:
         h.update(f.encode())
         h.update((CSRC / f).read_bytes())
     return h.hexdigest()[:16]
 
 
 def _compile_cmd(hipcc: str, src: str, obj: Path, defs: list) -> list:
-    cmd = [hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", *defs, *(NO_PACKED_FP32 if src in TOKEN_SOURCES else []), "-c", str(CSRC / src), "-o", str(obj)]
+    cmd = [hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", *defs, *NO_PACKED_FP32, "-c", str(CSRC / src), "-o", str(obj)]
     if src in NO_CONTRACT:
         cmd.insert(4, "-ffp-contract=off")
     if src in ("post.hip", "preproc.hip"):   # bit-exact box rescaling divides by the gain: IEEE division (hipcc's default, stated explicitly)
