@@ -4,13 +4,15 @@
 //     y  = x W^T    N = output channels (rows of W[e], K contiguous)         M = rows of x (K contiguous)          K = Cin
 //     dx = dy W     N = input channels (columns of W[e], N contiguous)       M = rows of dy (K contiguous)         K = Cout
 //     dW = dy^T x   N = input channels (columns of x, N contiguous)          M = output channels (columns of dy)   K = the expert's rows
-// A k-step takes 64 bytes of K per row of a K-contiguous side, and as many rows of a side whose own index is contiguous: either way a side's tile
-// of a k-step is 64 * TILE bytes.  Both are brought straight into LDS (`buffer_load_dwordx4 ... lds`), whatever lies outside the matrix as lanes out
-// of the buffer's range, which the hardware answers with zeros; so tails of rows, channels and K cost no other code.  A ring of four stages keeps
-// three k-steps of transfers in flight across one barrier a k-step (counted vmcnt), and the fragments of the next k-step are read while the matrix
-// instructions of this one run.
+// A k-step takes 128 bytes of K per row of a K-contiguous side (whole cache lines: with 64-byte steps the same bytes took twice the requests and the
+// transfers alone ran at 10 instead of 13 TB/s), and as many rows of a side whose own index is contiguous: either way a side's tile of a k-step is
+// 128 * TILE bytes.  Both are brought straight into LDS (`buffer_load_dwordx4 ... lds`), whatever lies outside the matrix as lanes out of the
+// buffer's range, which the hardware answers with zeros; so tails of rows, channels and K cost no other code.  A k-step is multiplied in two
+// halves: while the matrix instructions of one run, the fragments of the next are read into the other half of the registers.  A side's tile of a step is
+// a unit of a ring of five: the M side's unit of a step is brought during an earlier step's second half and the N side's during a first half, so that
+// transfers (and their LDS writes) go on evenly all the time, two to three halves ahead, with one barrier a step.
 //
-// Fragments are those of the 32 x 32 matrix instructions: lane l holds row l % 32 and the 16-byte pieces l / 32 and 2 + l / 32 of its 64 bytes — the
+// Fragments are those of the 32 x 32 matrix instructions: lane l holds row l % 32 and the 16-byte pieces l / 32 and 2 + l / 32 of a half's 64 bytes — the
 // order of K within a k-step is free as long as both sides use the same.  A side whose own index is contiguous is read through the transposing LDS
 // load (16-bit) or element by element (fp32).  The N side's rows are permuted so that the 16 results a lane holds of a 32 x 32 block are 16
 // CONSECUTIVE output channels (16-byte stores): row i of the block is channel ((i >> 2) & 1) * 16 + (i >> 3) * 4 + (i & 3).
@@ -24,7 +26,12 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-#define EX_STAGES 4
+#define EX_UNITS 5
+#ifdef YMK_HOST_EMU
+#define EX_SCHED_FENCE() ((void)0)
+#else
+#define EX_SCHED_FENCE() __builtin_amdgcn_sched_barrier(0)
+#endif
 
 namespace {
 
@@ -84,6 +91,39 @@ __device__ __forceinline__ f32x16 ex_mfma(const ExFrag& a, const ExFrag& b, f32x
     }
 }
 
+// c + the elements of a fragment
+template <typename T>
+__device__ __forceinline__ float ex_sum(const ExFrag& f, float c) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = f.p[q][i];
+            if constexpr (sizeof(T) == 4) c += __uint_as_float(w);
+            else c = dot2_h16(w, pack_h16x2(1.f, 1.f), c);
+        }
+    return c;
+}
+
+// A raw buffer at p (an offset with bit 31 set is out of its range: zeros, no access), and 16 bytes a lane from it to LDS at dst (wave-uniform) + lane * 16.
+// The transfer is written as assembly because the compiler waits for ALL transfers before any transposing LDS read when it knows of them (dx of 32768 x
+// 4096 by 1024 in bf16: 530 us).  It has no register result; this kernel's counted waits and barriers order it against the reads of its bytes.
+#ifdef YMK_HOST_EMU
+typedef hostemu_rsrc ExBuffer;
+__device__ __forceinline__ ExBuffer ex_buffer(const char* p) { return GLDS_MAKE_RSRC(p, 0x7fffffff); }
+__device__ __forceinline__ void ex_load_lds(const ExBuffer& b, char* dst, unsigned voff) { GLDS_BUFFER_LOAD_LDS(b, dst, voff, 0); }
+#else
+typedef u32x4 ExBuffer;
+__device__ __forceinline__ ExBuffer ex_buffer(const char* p) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    return ExBuffer{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
+}
+__device__ __forceinline__ void ex_load_lds(const ExBuffer& b, char* dst, unsigned voff) {
+    // five wait states: M0 written by the scalar unit needs one, a scalar register written by a vector instruction (the buffer's) five
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"((uint32_t)(uintptr_t)(glds_lptr)dst), "v"(voff), "s"(b) : "memory", "m0");
+}
+#endif
+
 __device__ __forceinline__ u32x2 ex_read_tr(const char* p) {
 #ifdef YMK_HOST_EMU
     return hostemu_ds_read_tr16_b64(p);
@@ -97,29 +137,31 @@ __device__ __forceinline__ int ex_perm(int i) { return ((i >> 2) & 1) * 16 + (i 
 
 // One side's tile in LDS.  KC: K contiguous.
 // `spread`: rows permuted (the N side; the transposing reader permutes its columns by itself, for either side).
-//   KC:  row r at r * 64, its 16-byte piece c in slot c ^ ((r >> 1) & 3): eight consecutive rows read at the same piece cover 128 bytes of banks
-//   !KC: k-row k at k * TILE * ES; 16-bit pieces c in slot c ^ ((k & 1) | (k & 2) << 1): the four k-rows a transposing read takes at once do
+//   KC:  row r at r * 128, its 16-byte piece c in slot c ^ ((r >> 1) & 7): the 16 rows that a 16-byte read serves at once (0-3, 12-15, 20-23, 24-27 and
+//        their complement, or 16 in a row) cover all 64 banks
+//   !KC: k-row k at k * TILE * ES; 16-bit pieces c in slot c ^ ((k & 3) << 2): the four k-rows by 64 bytes that half a wave's transposing read takes do
 template <typename T, bool KC, int TILE>
 struct ExSide {
-    static constexpr int ES = ExElem<T>::ES, WT = TILE / 64, KS = 64 / ES;
-    static constexpr int LPR = KC ? 4 : TILE * ES / 16;   // lanes (16-byte pieces) of an LDS row
-    static constexpr int RPI = 64 / LPR;                  // rows a wave brings with one instruction (0 is impossible: TILE * ES <= 1024)
+    static constexpr int ES = ExElem<T>::ES, KS = 128 / ES;   // elements of K a step
+    static constexpr int LPR = KC ? 8 : TILE * ES / 16;        // lanes (16-byte pieces) of an LDS row
+    static constexpr int RPI = 64 / LPR;                       // rows a wave brings with one transfer (TILE * ES <= 1024)
+    static constexpr int LOADS = TILE / 32;                    // transfers of a wave a step
 
     const char* base;
-    unsigned voff[WT];
-    int32_t ld, K, kpiece, krow[WT];
+    unsigned voff[LOADS];
+    int32_t ld, K, kfirst[KC ? 1 : LOADS];
 
-    // first / limit: rows (KC) or elements (!KC) of the tile's own index from `base`'s origin; K in elements
+    // first / limit: the tile's own index, counted from `origin`; K in elements
     __device__ __forceinline__ void init(const char* origin, int32_t ld_, int first, int limit, int K_, bool spread, int wave, int lane) {
         ld = ld_;
         K = K_;
         const int lr = lane / LPR, pc = lane % LPR;
         if constexpr (KC) {
-            const int sc = pc ^ ((lr >> 1) & 3);
+            const int sc = pc ^ ((((wave & 1) * 8 + lr) >> 1) & 7);   // row (j * 4 + wave) * 8 + lr
             base = origin + (int64_t)first * ld;
-            kpiece = sc * (16 / ES);
+            kfirst[0] = sc * (16 / ES);
 #pragma unroll
-            for (int j = 0; j < WT; ++j) {
+            for (int j = 0; j < LOADS; ++j) {
                 int r = (j * 4 + wave) * RPI + lr;
                 if (spread) r = (r & ~31) + ex_perm(r & 31);
                 voff[j] = first + r < limit ? (unsigned)(r * ld + sc * 16) : 0x80000000u;
@@ -127,46 +169,45 @@ struct ExSide {
         } else {
             base = origin + (int64_t)first * ES;
 #pragma unroll
-            for (int j = 0; j < WT; ++j) {
+            for (int j = 0; j < LOADS; ++j) {
                 const int k = (j * 4 + wave) * RPI + lr;
-                const int sc = ES == 2 ? pc ^ ((k & 1) | ((k & 2) << 1)) : pc;
-                krow[j] = k;
+                const int sc = ES == 2 ? pc ^ ((k & 3) << 2) : pc;
+                kfirst[j] = k;
                 voff[j] = first + sc * (16 / ES) < limit ? (unsigned)(k * ld + sc * 16) : 0x80000000u;
             }
         }
     }
-    // bring k-step `step` to `dst` (this side's part of a stage); steps behind the last one bring zeros
-    __device__ __forceinline__ void issue(int step, char* dst, int wave) const {
-        const char* b = base + (KC ? (int64_t)step * 64 : (int64_t)step * KS * ld);
-        const glds_rsrc rs = GLDS_MAKE_RSRC(b, 0x7fffffff);
-        const int left = K - step * KS;
-#pragma unroll
-        for (int j = 0; j < WT; ++j) {
-            const unsigned out = (KC ? kpiece : krow[j]) < left ? 0u : 0x80000000u;
-            GLDS_BUFFER_LOAD_LDS(rs, dst + (j * 4 + wave) * 1024, voff[j] | out, 0);
-        }
+    // k-step `step` as a buffer; steps behind the last one bring zeros
+    struct Step { ExBuffer rs; int left; };
+    __device__ __forceinline__ Step at(int step) const {
+        return {ex_buffer(base + (KC ? (int64_t)step * 128 : (int64_t)step * KS * ld)), K - step * KS};
     }
-    // fragment of the 32 rows at `r0` of the tile
-    static __device__ __forceinline__ ExFrag read(const char* src, int r0, int lane) {
+    // bring transfer j of it to `dst` (this side's part of a slot)
+    __device__ __forceinline__ void issue(const Step& s, int j, char* dst, int wave) const {
+        const unsigned out = kfirst[KC ? 0 : j] < s.left ? 0u : 0x80000000u;
+        ex_load_lds(s.rs, dst + (j * 4 + wave) * 1024, voff[j] | out);
+    }
+    // fragment of the 32 rows at `r0` of the tile, half `half` of the step
+    static __device__ __forceinline__ ExFrag read(const char* src, int r0, int half, int lane) {
         ExFrag f;
         if constexpr (KC) {
-            const int r = r0 + (lane & 31), s = (r >> 1) & 3, h = lane >> 5;
-            f.p[0] = *reinterpret_cast<const u32x4*>(src + r * 64 + ((h ^ s) * 16));
-            f.p[1] = *reinterpret_cast<const u32x4*>(src + r * 64 + (((2 + h) ^ s) * 16));
+            const int r = r0 + (lane & 31), s = (r >> 1) & 7, c = half * 4 + (lane >> 5);
+            f.p[0] = *reinterpret_cast<const u32x4*>(src + r * 128 + ((c ^ s) * 16));
+            f.p[1] = *reinterpret_cast<const u32x4*>(src + r * 128 + (((c + 2) ^ s) * 16));
         } else if constexpr (ES == 2) {
             // 16 lanes read four k-rows of 16 elements, four lanes a row and 8 bytes a lane, and each gets one column: k-row (lane % 16) / 4,
             // elements of the permuted columns 4 * (lane % 4) .. + 3 of this half of the block
             const int i = lane & 15, g = (lane >> 4) & 1, h = lane >> 5, q = i & 3, kk = i >> 2;
             const int col = r0 + (q & 1) * 16 + (2 * g + (q >> 1)) * 4;
-            const int slot = (col >> 3) ^ ((kk & 1) | ((kk & 2) << 1));
-            const char* p = src + (h * 8 + kk) * (TILE * 2) + slot * 16 + (col & 4) * 2;
+            const int slot = (col >> 3) ^ (kk << 2);
+            const char* p = src + (half * 32 + h * 8 + kk) * (TILE * 2) + slot * 16 + (col & 4) * 2;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const u32x2 lo = ex_read_tr(p + (c * 16) * (TILE * 2)), hi = ex_read_tr(p + (c * 16 + 4) * (TILE * 2));
                 f.p[c] = u32x4{lo.x, lo.y, hi.x, hi.y};
             }
         } else {
-            const char* p = src + ((lane >> 5) * 4) * (TILE * 4) + (r0 + ex_perm(lane & 31)) * 4;
+            const char* p = src + (half * 16 + (lane >> 5) * 4) * (TILE * 4) + (r0 + ex_perm(lane & 31)) * 4;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -220,17 +261,35 @@ __device__ __forceinline__ bool ex_find(const ExArgs& a, ExTile& t) {
     return false;
 }
 
-__device__ __forceinline__ float ex_act(float v, int act) {
-    if (act == YMK_ACT_SILU) return silu_exact(v);
-    if (act == YMK_ACT_GELU) return gelu_exact(v);
-    if (act == YMK_ACT_SIGMOID) return sigmoid_exact(v);
-    return v;
+// The activation of an fp32 output in the exact forms; of a 16-bit one in short forms of a few units of 2^-23 (the exact ones take about 50 instructions an
+// element, more than the products of a 2048-wide row).  GELU = x Phi(x) through erfc(z) = t exp(-z^2 + p(t)), t = 1 / (1 + z / 2): the Chebyshev fit
+// of Press et al., Numerical Recipes (2nd ed., 6.2), relative error 1.2e-7 everywhere, so the negative tail keeps its digits.
+template <int ACT, bool SHORT>
+__device__ __forceinline__ float ex_act(float v) {
+    if constexpr (ACT == YMK_ACT_SILU) return SHORT ? silu_f(v) : silu_exact(v);
+    else if constexpr (ACT == YMK_ACT_SIGMOID) return SHORT ? __builtin_amdgcn_rcpf(1.0f + __expf(-v)) : sigmoid_exact(v);
+    else if constexpr (ACT == YMK_ACT_GELU) {
+        if constexpr (!SHORT) return gelu_exact(v);
+        const float z = fabsf(v) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(z, 0.5f, 1.0f));
+        float p = 0.17087277f;
+        p = fmaf(p, t, -0.82215223f);
+        p = fmaf(p, t, 1.48851587f);
+        p = fmaf(p, t, -1.13520398f);
+        p = fmaf(p, t, 0.27886807f);
+        p = fmaf(p, t, -0.18628806f);
+        p = fmaf(p, t, 0.09678418f);
+        p = fmaf(p, t, 0.37409196f);
+        p = fmaf(p, t, 1.00002368f);
+        p = fmaf(p, t, -1.26551223f);
+        const float half_erfc = 0.5f * t * __expf(fmaf(-z, z, p));
+        return v > 0.f ? v - v * half_erfc : v * half_erfc;
+    } else return v;
 }
 
 // NKC / MKC: K contiguous on that side.  DW: K is the expert's rows.  TO: output type.
 template <typename T, typename TO, bool NKC, bool MKC, int TILE, bool DB>
 __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K, const char* nsrc, const char* msrc) {
-    constexpr int WT = TILE / 64, SIDE = TILE * 64, STAGE = 2 * SIDE, LOADS = 2 * WT;
+    constexpr int WT = TILE / 64, UNIT = TILE * 128, LOADS = TILE / 32, CHUNKS = 2 * WT;
     extern __shared__ u32x4 ex_lds[];
     char* lds = reinterpret_cast<char*>(ex_lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wn = wave & 1, wm = wave >> 1;
@@ -240,12 +299,21 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
     MSide ms;
     ns.init(nsrc, a.n_ld, t.n0, a.N, K, true, wave, lane);
     ms.init(msrc, a.m_ld, t.m0, t.mend, K, false, wave, lane);
-    auto issue = [&](int step) {
-        char* dst = lds + (step & (EX_STAGES - 1)) * STAGE;
-        ns.issue(step, dst, wave);
-        ms.issue(step, dst + SIDE, wave);
-    };
-    f32x16 acc[WT][WT], accb[DB ? WT : 1];
+    constexpr int CH = WT * 32, LPR = CH / 8, RPI = 64 / LPR;   // a wave's channels, the lanes of an output row and the rows of a store
+    const int c0 = t.n0 + wn * CH + (lane % LPR) * 8;
+    float bias[8], scale[8], mscale[WT];   // fetched here: their latency is not the epilogue's
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        bias[e] = a.bias && c0 + e < a.N ? a.bias[(int64_t)t.e * a.N + c0 + e] : 0.f;
+        scale[e] = a.n_scale && c0 + e < a.N ? a.n_scale[(int64_t)t.e * a.N + c0 + e] : 1.f;
+    }
+#pragma unroll
+    for (int j = 0; j < WT; ++j) {
+        const int row = t.m0 + (wm * WT + j) * 32 + (lane & 31);
+        mscale[j] = a.m_scale && row < t.mend ? a.m_scale[row] : 1.f;
+    }
+    f32x16 acc[WT][WT];
+    float accb[WT];   // DB: this lane's part of the sum over K of its M-side rows
 #pragma unroll
     for (int i = 0; i < WT; ++i)
 #pragma unroll
@@ -253,98 +321,128 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 #pragma unroll
-    for (int j = 0; j < (DB ? WT : 1); ++j)
+    for (int j = 0; j < WT; ++j) accb[j] = 0.f;
+    ExFrag fn[2][WT], fm[2][WT];   // the fragments of a step's two halves
+    const int steps = (K + NSide::KS - 1) / NSide::KS;
+    // Units in the order they are brought: N of step 0, M of step 0, N of 1, ...; unit u lies at (u % 5) * UNIT.  Step k's are free once every wave has the
+    // fragments of its second half, which the barrier between the halves of step k says.  Before it unit 2 k + 4 (N of k + 2) may be brought, to where M
+    // of k - 1 was; after it unit 2 k + 5 (M of k + 2), to where N of k was.  At the barrier all units up to 2 k + 3 have to have landed: those of step
+    // k + 1, whose first half is read next.
+    int un = 0;   // (2 k) % 5
+    auto unit = [&](int u) { return lds + (u >= EX_UNITS ? u - EX_UNITS : u) * UNIT; };
 #pragma unroll
-        for (int r = 0; r < 16; ++r) accb[j][r] = 0.f;
-    ExFrag ones;   // 1 in every element: the sum over K of the M side as a matrix product
+    for (int q = 0; q < 2; ++q) {
+        const auto n = ns.at(q);
+        const auto m = ms.at(q);
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+        for (int j = 0; j < LOADS; ++j) ns.issue(n, j, lds + 2 * q * UNIT, wave);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ones.p[c][i] = sizeof(T) == 4 ? 0x3f800000u : pack_h16x2(1.f, 1.f);
-    ExFrag fn[2][WT], fm[2][WT];
-    auto read = [&](int step, ExFrag (&n)[WT], ExFrag (&m)[WT]) {
-        const char* src = lds + (step & (EX_STAGES - 1)) * STAGE;
-#pragma unroll
-        for (int i = 0; i < WT; ++i) n[i] = NSide::read(src, (wn * WT + i) * 32, lane);
-#pragma unroll
-        for (int j = 0; j < WT; ++j) m[j] = MSide::read(src + SIDE, (wm * WT + j) * 32, lane);
-    };
-    const int nk = (K + NSide::KS - 1) / NSide::KS;
-    // Stage k + 1 has to have landed for every wave, and every wave has to have its fragments of stage k in registers, before stage k's slot is
-    // given to stage k + 4 and the fragments of stage k + 1 are read.
-#pragma unroll
-    for (int s = 0; s < EX_STAGES; ++s) issue(s);
-    __builtin_amdgcn_s_waitcnt(GLDS_WAITCNT_VM((EX_STAGES - 1) * LOADS));
+        for (int j = 0; j < LOADS; ++j) ms.issue(m, j, lds + (2 * q + 1) * UNIT, wave);
+    }
+    __builtin_amdgcn_s_waitcnt(GLDS_WAITCNT_VM(2 * LOADS));
     GLDS_COMPILER_FENCE();
     __builtin_amdgcn_s_barrier();
     GLDS_COMPILER_FENCE();
-    read(0, fn[0], fm[0]);
-    auto step = [&](int k, ExFrag (&n)[WT], ExFrag (&m)[WT], ExFrag (&n2)[WT], ExFrag (&m2)[WT]) {
-        __builtin_amdgcn_s_waitcnt(GLDS_WAITCNT_VM((EX_STAGES - 2) * LOADS));
+#pragma unroll
+    for (int i = 0; i < WT; ++i) {
+        fn[0][i] = NSide::read(lds, (wn * WT + i) * 32, 0, lane);
+        fm[0][i] = MSide::read(lds + UNIT, (wm * WT + i) * 32, 0, lane);
+    }
+    // The matrix instructions of half `h` with, between every few of them, the reads of one fragment of the next half and a transfer, in this order: left
+    // to itself the compiler moves the matrix instructions (they need no memory) to the reads of their own fragments, and the transfers before them all.
+    auto half = [&](auto H, const char* nsrc_, const char* msrc_, char* dst, const auto& next) {
+        constexpr int h = decltype(H)::value;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            EX_SCHED_FENCE();
+#pragma unroll
+            for (int q = c * (WT * WT) / CHUNKS; q < (c + 1) * (WT * WT) / CHUNKS; ++q)
+                acc[q / WT][q % WT] = ex_mfma<T>(fn[h][q / WT], fm[h][q % WT], acc[q / WT][q % WT]);
+            EX_SCHED_FENCE();
+#pragma unroll
+            for (int j = c * LOADS / CHUNKS; j < (c + 1) * LOADS / CHUNKS; ++j) {
+                if constexpr (h == 0) ns.issue(next, j, dst, wave);
+                else ms.issue(next, j, dst, wave);
+            }
+            if (c < WT) {
+                fn[1 - h][c] = NSide::read(nsrc_, (wn * WT + c) * 32, 1 - h, lane);
+                if constexpr (DB) accb[c] = ex_sum<T>(fm[h][c], accb[c]);
+            } else {
+                fm[1 - h][c - WT] = MSide::read(msrc_, (wm * WT + c - WT) * 32, 1 - h, lane);
+            }
+        }
+        EX_SCHED_FENCE();
+    };
+    for (int k = 0; k < steps; ++k) {
+        half(std::integral_constant<int, 0>{}, unit(un), unit(un + 1), unit(un + 4), ns.at(k + 2));
+        __builtin_amdgcn_s_waitcnt(GLDS_WAITCNT_VM(LOADS));   // all but the unit that was brought last
         GLDS_WAIT_LGKM0();
         __builtin_amdgcn_s_barrier();
         GLDS_COMPILER_FENCE();
-        issue(k + EX_STAGES);
-        read(k + 1, n2, m2);
-#pragma unroll
-        for (int i = 0; i < WT; ++i)
-#pragma unroll
-            for (int j = 0; j < WT; ++j) acc[i][j] = ex_mfma<T>(n[i], m[j], acc[i][j]);
-        if constexpr (DB) {
-#pragma unroll
-            for (int j = 0; j < WT; ++j) accb[j] = ex_mfma<T>(ones, m[j], accb[j]);
-        }
-    };
-    for (int k = 0; k < nk; k += 2) {   // a step behind the last one multiplies zeros
-        step(k, fn[0], fm[0], fn[1], fm[1]);
-        step(k + 1, fn[1], fm[1], fn[0], fm[0]);
+        half(std::integral_constant<int, 1>{}, unit(un + 2), unit(un + 3), unit(un), ms.at(k + 2));
+        un = un + 2 >= EX_UNITS ? un + 2 - EX_UNITS : un + 2;
     }
-    __builtin_amdgcn_s_waitcnt(GLDS_WAITCNT_VM(0));   // no transfer may reach LDS after the workgroup has ended
+    __builtin_amdgcn_s_waitcnt(GLDS_WAITCNT_VM(0));   // the transfers of zeros behind the last step have landed: LDS is free once every wave is here
+    __syncthreads();
 
-    // lane l: output row l % 32 of block j (permuted like the N side where the M side's own index is contiguous), 16 channels of block i
+    // Lane l holds output row l % 32 of block j (permuted like the N side where the M side's own index is contiguous) and 16 channels of block i.
+    // A wave turns one block of 32 rows at a time through its own part of LDS, so that a row leaves as whole lines and the scales, the bias and
+    // the activation are code of a short loop (inlined per accumulator they would overflow the instruction cache).
+    constexpr int LD = CH + 4;   // 16 bytes of padding: eight rows written at once meet eight different banks
+    float* turn = reinterpret_cast<float*>(lds) + wave * (32 * LD);
+    static_assert(4 * 32 * LD * 4 <= EX_UNITS * UNIT, "the turning buffers fit the units");
     const int h = lane >> 5;
     TO* out = reinterpret_cast<TO*>(a.out + (MKC ? 0 : t.e * a.out_expert));
 #pragma unroll
     for (int j = 0; j < WT; ++j) {
-        const int row = t.m0 + (wm * WT + j) * 32 + (MKC ? lane & 31 : ex_perm(lane & 31));
-        if (row >= t.mend) continue;
+        const int row0 = t.m0 + (wm * WT + j) * 32;
+        if (row0 >= t.mend) break;
         if constexpr (DB) {
-            if (wn == 0 && h == 0) a.db[(int64_t)t.e * a.M + row] = accb[j][0];
+            const int row = row0 + (MKC ? lane & 31 : ex_perm(lane & 31));
+            const float sum = accb[j] + __shfl_xor(accb[j], 32);   // lanes l and l + 32 hold the same row's other halves of K
+            if (wn == 0 && h == 0 && row < t.mend) a.db[(int64_t)t.e * a.M + row] = sum;
         }
-        const float ms_ = a.m_scale ? a.m_scale[row] : 1.f;
+        float* w = turn + (MKC ? lane & 31 : ex_perm(lane & 31)) * LD + h * 16;
 #pragma unroll
-        for (int i = 0; i < WT; ++i) {
-            const int ch = t.n0 + (wn * WT + i) * 32 + h * 16;
+        for (int i = 0; i < WT; ++i)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int c = ch + q * 8;
-                if (c >= a.N) continue;   // N is a multiple of 8 (fp32: of 4)
-                float v[8];
-                const bool tail = sizeof(TO) == 4 && c + 4 >= a.N;   // only the first four exist
+            for (int q = 0; q < 4; ++q) {
+                float v[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = acc[i][j][q * 8 + e];
-                if (a.n_scale) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] *= ms_ * a.n_scale[(int64_t)t.e * a.N + c + e];
-                }
-                if (a.bias) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e < 4 || !tail) v[e] += a.bias[(int64_t)t.e * a.N + c + e];
-                }
-                if (a.act != YMK_ACT_NONE) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = ex_act(v[e], a.act);
-                }
-                TO* p = out + (int64_t)row * a.out_ld + c;
-                if constexpr (sizeof(TO) == 4) {
-                    store4(reinterpret_cast<float*>(p), v[0], v[1], v[2], v[3]);
-                    if (!tail) store4(reinterpret_cast<float*>(p) + 4, v[4], v[5], v[6], v[7]);
-                } else {
-                    store_vec_f32(p, v);
-                }
+                for (int e = 0; e < 4; ++e) v[e] = std::is_same<T, E4m3>::value ? acc[i][j][q * 4 + e] * mscale[j] : acc[i][j][q * 4 + e];
+                store4(w + i * 32 + q * 4, v[0], v[1], v[2], v[3]);
             }
-        }
+        __builtin_amdgcn_wave_barrier();   // only this wave's part: LDS operations of a wave stay in order
+        auto some = [&](int r0, auto ACT) {   // RPI rows
+            const int r = r0 + lane / LPR, row = row0 + r;
+            float v[8];
+            load4(turn + r * LD + (lane % LPR) * 8, v[0], v[1], v[2], v[3]);
+            load4(turn + r * LD + (lane % LPR) * 8 + 4, v[4], v[5], v[6], v[7]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = std::is_same<T, E4m3>::value ? fmaf(v[e], scale[e], bias[e]) : v[e] + bias[e];
+                v[e] = ex_act<decltype(ACT)::value, sizeof(TO) == 2>(v[e]);
+            }
+            if (row >= t.mend || c0 >= a.N) return;
+            TO* p = out + (int64_t)row * a.out_ld + c0;
+            if constexpr (sizeof(TO) == 4) {
+                store4(reinterpret_cast<float*>(p), v[0], v[1], v[2], v[3]);
+                if (c0 + 4 < a.N) store4(reinterpret_cast<float*>(p) + 4, v[4], v[5], v[6], v[7]);   // fp32 channels come in fours, the others in eights
+            } else {
+                store_vec_f32(p, v);
+            }
+        };
+        auto block = [&](auto ACT) {
+#pragma unroll 2
+            for (int r0 = 0; r0 < 32; r0 += RPI) some(r0, ACT);
+        };
+        if (!MKC || !NKC || a.act == YMK_ACT_NONE) {
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += RPI) some(r0, std::integral_constant<int, YMK_ACT_NONE>{});
+        } else if (a.act == YMK_ACT_SILU) block(std::integral_constant<int, YMK_ACT_SILU>{});
+        else if (a.act == YMK_ACT_GELU) block(std::integral_constant<int, YMK_ACT_GELU>{});
+        else block(std::integral_constant<int, YMK_ACT_SIGMOID>{});
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -359,12 +457,15 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void expert_rows_kernel(E
 // dW (and, by the workgroups of the first channels, db)
 template <typename T, typename TO, int TILE>
 __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void expert_dw_kernel(ExArgs a) {
-    const int nt = (a.N + TILE - 1) / TILE, mt = (a.M + TILE - 1) / TILE, per = (gridDim.x + 7) / 8;
-    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (id >= a.E * nt * mt) return;
+    // Experts differ in rows, so each expert's tiles are split over all XCDs: eight runs of neighbouring tiles, one an XCD (32768 rows over 8 experts
+    // drawn with a spread of 0.3, 1024 by 4096: an expert an XCD took 324 us, this 278 us); fewer than eight tiles go round in turn.
+    const int nt = (a.N + TILE - 1) / TILE, mt = (a.M + TILE - 1) / TILE, all = nt * mt, run = (all + 7) / 8;
+    const int slot = all < 8 ? blockIdx.x : blockIdx.x >> 3;
     ExTile t;
-    t.e = id / (nt * mt);
-    t.m0 = id / nt % mt * TILE;
+    t.e = slot / (all < 8 ? all : run);
+    const int id = all < 8 ? slot % all : (blockIdx.x & 7) * run + slot % run;
+    if (t.e >= a.E || id >= all) return;
+    t.m0 = id / nt * TILE;
     t.mend = a.M;
     t.n0 = id % nt * TILE;
     const int first = min(max(a.offsets[t.e], 0), a.rows), last = min(max(a.offsets[t.e + 1], first), a.rows);
@@ -393,16 +494,24 @@ inline int64_t ex_blocks(int64_t rows, int E, int N, int tile) {
     return (mt * nt + 7) / 8 * 8;
 }
 
+// Tiles of 256 halve the bytes that reach LDS for a product, but leave CUs idle when there are few and waste rows when experts have few
+// (bf16, 32768 rows 4096 -> 4096 over 8 experts: 1009 us against 1159; 4096 rows 512 -> 2048 over 16: 22.8 against 24.6; e4m3, 4096 rows 1024 -> 2048
+// over 32: 40.2 against 28.1): from 192 rows an expert and one tile a CU on.
+inline bool ex_wide(int64_t rows, int E, int N) { return rows >= 192ll * E && (rows / 256 + E / 2) * ((N + 255) / 256) >= 256; }
+
 template <typename T, typename TO, bool NKC>
 int ex_rows(const ExArgs& a, void* stream) {
-    constexpr int TILE = 128;
-    return ex_launch<expert_rows_kernel<T, TO, NKC, TILE>>(a, ex_blocks(a.rows, a.E, a.N, TILE), EX_STAGES * 2 * TILE * 64, stream);
+    if (ex_wide(a.rows, a.E, a.N)) return ex_launch<expert_rows_kernel<T, TO, NKC, 256>>(a, ex_blocks(a.rows, a.E, a.N, 256), EX_UNITS * 256 * 128, stream);
+    return ex_launch<expert_rows_kernel<T, TO, NKC, 128>>(a, ex_blocks(a.rows, a.E, a.N, 128), EX_UNITS * 128 * 128, stream);
+}
+inline int64_t ex_dw_blocks(const ExArgs& a, int tile) {
+    const int64_t all = (int64_t)((a.N + tile - 1) / tile) * ((a.M + tile - 1) / tile);
+    return all < 8 ? all * a.E : (all + 7) / 8 * 8 * a.E;
 }
 template <typename T, typename TO>
 int ex_dw(const ExArgs& a, void* stream) {
-    constexpr int TILE = 128;
-    const int64_t blocks = (int64_t)a.E * ((a.N + TILE - 1) / TILE) * ((a.M + TILE - 1) / TILE);
-    return ex_launch<expert_dw_kernel<T, TO, TILE>>(a, (blocks + 7) / 8 * 8, EX_STAGES * 2 * TILE * 64, stream);
+    if (ex_dw_blocks(a, 256) >= 512) return ex_launch<expert_dw_kernel<T, TO, 256>>(a, ex_dw_blocks(a, 256), EX_UNITS * 256 * 128, stream);
+    return ex_launch<expert_dw_kernel<T, TO, 128>>(a, ex_dw_blocks(a, 128), EX_UNITS * 128 * 128, stream);
 }
 
 inline bool ex_bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15); }

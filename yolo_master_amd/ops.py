@@ -113,7 +113,8 @@ def conv_kernel_name(variant: int, dtype, cin: int, cout: int, k: int, kpad: int
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """torch.cuda.current_stream().cuda_stream, without the stream object (1.2 us of a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t: torch.Tensor | None):
@@ -706,6 +707,8 @@ def _timed(family: str, flops=None):
     def wrap(fn):
         @functools.wraps(fn)
         def run(*a, **kw):
+            if not TIMER.on:
+                return fn(*a, **kw)
             e0 = TIMER.begin()
             r = fn(*a, **kw)
             if e0 is not None:
@@ -1198,12 +1201,13 @@ _ROW_ACT = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "
 
 def _rows(t: torch.Tensor, what: str):
     """(rows, C, ld) of a row view."""
-    if t.dim() == 2:
-        M, Cc = t.shape
-        ld = t.stride(0)
-    elif t.dim() > 2:
-        Cc, M, ld = t.shape[-1], 1, 0
-        for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    shape, strides = t.shape, t.stride()
+    if len(shape) == 2:
+        M, Cc = shape
+        ld, dense = strides
+    elif len(shape) > 2:
+        Cc, M, ld, dense = shape[-1], 1, 0, strides[-1]
+        for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
             if n == 1:
                 continue
             if M == 1:
@@ -1212,8 +1216,8 @@ def _rows(t: torch.Tensor, what: str):
                 raise ValueError(f"{what}: the rows of the view are not evenly spaced")
             M *= n
     else:
-        raise ValueError(f"{what}: expected [..., C], got {tuple(t.shape)}")
-    if Cc > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: expected [..., C], got {tuple(shape)}")
+    if dense != 1 and Cc > 1:
         raise ValueError(f"{what}: the last dim must be dense")
     if M <= 1:
         return M, Cc, Cc
@@ -1224,25 +1228,41 @@ def _rows(t: torch.Tensor, what: str):
 
 def _here(what: str, first: torch.Tensor, *others) -> None:
     """All operands on one GPU, and that the current one (the call goes to its current stream)."""
-    require_gpu(first, what)
-    dev = first.device
+    dev = first.get_device()
+    if dev < 0:
+        require_gpu(first, what)
+    elif dev != torch.cuda.current_device():
+        raise ValueError(f"{what}: operands on {first.device}, current device cuda:{torch.cuda.current_device()}")
     for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: operands on {dev} and {t.device}")
-    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: operands on {dev}, current device cuda:{torch.cuda.current_device()}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: operands on {first.device} and {t.device}")
 
 
 def _fp32_vec(t, shape, what: str, name: str) -> None:
-    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: {name} is a contiguous fp32 {list(shape)} tensor, got {t.dtype} {list(t.shape)}")
 
 
 def _like(t, x, what: str, name: str):
     """t's row stride; t is a view of x's shape and dtype."""
-    if t.dtype != x.dtype or t.shape != x.shape:
+    if t.dtype is not x.dtype or t.shape != x.shape:
         raise ValueError(f"{what}: {name} is {t.dtype} {list(t.shape)}, expected {x.dtype} {list(x.shape)}")
     return _rows(t, what)[2]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _new(x, dtype):
+    """A dense tensor of x's shape."""
+    return torch.empty_like(x, dtype=dtype) if x.is_contiguous() else torch.empty(x.shape, dtype=dtype, device=x.device)
+
+
+def _new_stat(x, M: int, fp32):
+    """An fp32 value a row (fp32: any fp32 tensor of the device)."""
+    t = fp32.new_empty(M)
+    return t if x.dim() == 2 else t.view(x.shape[:-1])
 
 
 def _norm_args(what, x, weight, residual, residual_out):
@@ -1260,7 +1280,7 @@ def _norm_args(what, x, weight, residual, residual_out):
         return M, Cc, ldx, 0, x, 0
     ldr = _like(residual, x, what, "residual")
     if residual_out is None:
-        return M, Cc, ldx, ldr, torch.empty(x.shape, dtype=x.dtype, device=x.device), Cc
+        return M, Cc, ldx, ldr, _new(x, x.dtype), Cc
     ldh = _like(residual_out, x, what, "residual_out")
     for t, ld in ((x, ldx), (residual, ldr)):   # in place is fine, row by row; a shifted view is not
         a, b = t.data_ptr(), residual_out.data_ptr()
@@ -1275,10 +1295,9 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
     """h = x + residual (rounded to x's dtype; h is x without a residual), y = h / sqrt(mean(h^2) + eps) * weight.  Returns (y, h, rstd); rstd
     fp32, one a row, is what rms_norm_backward takes.  residual_out: where h goes (x or residual themselves, or a tensor apart from them)."""
     M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm", x, weight, residual, residual_out)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    check(lib.ymk_rms_norm(DT[x.dtype], _p(x), ldx, _p(residual), ldr, _p(h) if residual is not None else None, ldh, _p(y), Cc, _p(rstd), M, Cc, _p(weight),
-                           float(eps), _stream()), "rms_norm")
+    y, rstd = _new(x, x.dtype), _new_stat(x, M, weight)
+    check(lib.ymk_rms_norm(DT[x.dtype], x.data_ptr(), ldx, _ptr(residual), ldr, None if residual is None else h.data_ptr(), ldh, y.data_ptr(), Cc, rstd.data_ptr(),
+                           M, Cc, weight.data_ptr(), eps, _stream()), "rms_norm")
     return y, h, rstd
 
 
@@ -1287,10 +1306,9 @@ def rms_norm_quant(x, weight, eps: float = 1e-6, residual=None, residual_out=Non
     """The same norm with an 8-bit output: (q, scale, h), q e4m3 of x's shape and scale fp32 per row with y = q * scale, max |q| = 448
     (an all-zero row: scale 1; a row with a NaN or an infinity: all NaN)."""
     M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm_quant", x, weight, residual, residual_out)
-    q = torch.empty(x.shape, dtype=E4M3, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    check(lib.ymk_rms_norm_quant(DT[x.dtype], _p(x), ldx, _p(residual), ldr, _p(h) if residual is not None else None, ldh, _p(q), Cc, _p(scale), M, Cc,
-                                 _p(weight), float(eps), _stream()), "rms_norm_quant")
+    q, scale = _new(x, E4M3), _new_stat(x, M, weight)
+    check(lib.ymk_rms_norm_quant(DT[x.dtype], x.data_ptr(), ldx, _ptr(residual), ldr, None if residual is None else h.data_ptr(), ldh, q.data_ptr(), Cc,
+                                 scale.data_ptr(), M, Cc, weight.data_ptr(), eps, _stream()), "rms_norm_quant")
     return q, scale, h
 
 
@@ -1310,15 +1328,14 @@ def rms_norm_backward(dy, h, weight, rstd, dres=None, need_dweight: bool = True)
     lddy = _like(dy, h, what, "dy")
     lddr = _like(dres, h, what, "dres") if dres is not None else 0
     use_format(h.dtype)
-    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dx = _new(h, h.dtype)
     dweight = ws = None
     nbytes = 0
     if need_dweight:
-        dweight = torch.empty((Cc,), dtype=torch.float32, device=h.device)
         nbytes = lib.ymk_rms_norm_backward_workspace_bytes(M, Cc)
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=h.device)
-    check(lib.ymk_rms_norm_backward(DT[h.dtype], _p(dy), lddy, _p(h), ldh, _p(rstd), _p(weight), _p(dres), lddr, _p(dx), Cc, _p(dweight), M, Cc, _p(ws),
-                                    nbytes, _stream()), what)
+        dweight, ws = weight.new_empty(Cc), weight.new_empty(nbytes // 4)
+    check(lib.ymk_rms_norm_backward(DT[h.dtype], dy.data_ptr(), lddy, h.data_ptr(), ldh, rstd.data_ptr(), weight.data_ptr(), _ptr(dres), lddr, dx.data_ptr(), Cc,
+                                    _ptr(dweight), M, Cc, _ptr(ws), nbytes, _stream()), what)
     return dx, dweight
 
 
@@ -1341,13 +1358,12 @@ def token_sort(idx, experts: int) -> TokenPlan:
     T, K = idx.shape
     if not 1 <= K <= _lib.TOKEN_MAX_K or not 1 <= experts <= _lib.TOKEN_MAX_E or T * K >= 1 << 30:
         raise ValueError(f"token_sort: top_k {K} (1 .. {_lib.TOKEN_MAX_K}), {experts} experts (1 .. {_lib.TOKEN_MAX_E}), {T} tokens")
-    dev = idx.device
-    offsets = torch.empty((experts + 1,), dtype=torch.int32, device=dev)
-    src = torch.empty((T * K,), dtype=torch.int32, device=dev)
-    row = torch.empty((T, K), dtype=torch.int32, device=dev)
+    row = torch.empty_like(idx, dtype=torch.int32)
+    offsets, src = row.new_empty(experts + 1), row.new_empty(T * K)
     nbytes = lib.ymk_token_sort_workspace_bytes(T, K, experts)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
-    check(lib.ymk_token_sort(_p(idx), idx.element_size(), T, K, experts, _p(offsets), _p(src), _p(row), _p(ws), nbytes, _stream()), "token_sort")
+    ws = row.new_empty(nbytes // 4) if nbytes else None
+    check(lib.ymk_token_sort(idx.data_ptr(), idx.element_size(), T, K, experts, offsets.data_ptr(), src.data_ptr(), row.data_ptr(), _ptr(ws), nbytes, _stream()),
+          "token_sort")
     return TokenPlan(offsets, src, row, experts)
 
 
@@ -1367,13 +1383,14 @@ def token_dispatch(x, plan: TokenPlan, scale=None):
     _here("token_dispatch", x, plan.row, scale)
     T, K, Cc, ldx = _planned("token_dispatch", plan, x)
     es = x.element_size()
-    xs = torch.empty((T * K, Cc), dtype=x.dtype, device=x.device)
+    xs = x.new_empty(T * K, Cc)
     xs_scale = None
     if scale is not None:
         if scale.numel() != T or scale.dtype != torch.float32 or not scale.is_contiguous():
             raise ValueError(f"token_dispatch: scale is contiguous fp32, one a token ({T})")
-        xs_scale = torch.empty((T * K,), dtype=torch.float32, device=x.device)
-    check(lib.ymk_token_dispatch(_p(x), ldx * es, Cc * es, _p(scale), _p(xs), Cc * es, _p(xs_scale), _p(plan.row), T, K, _stream()), "token_dispatch")
+        xs_scale = scale.new_empty(T * K)
+    check(lib.ymk_token_dispatch(x.data_ptr(), ldx * es, Cc * es, _ptr(scale), xs.data_ptr(), Cc * es, _ptr(xs_scale), plan.row.data_ptr(), T, K, _stream()),
+          "token_dispatch")
     return xs if scale is None else (xs, xs_scale)
 
 
@@ -1385,8 +1402,8 @@ def _combine(what, ys, plan, w):
     if w is not None:
         _fp32_vec(w, (T, K), what, "w")
     use_format(ys.dtype)
-    y = torch.empty((T, Cc), dtype=ys.dtype, device=ys.device)
-    check(lib.ymk_token_combine(DT[ys.dtype], _p(ys), ldys, _p(plan.row), _p(w), _p(y), Cc, T, K, Cc, _stream()), what)
+    y = ys.new_empty(T, Cc)
+    check(lib.ymk_token_combine(DT[ys.dtype], ys.data_ptr(), ldys, plan.row.data_ptr(), _ptr(w), y.data_ptr(), Cc, T, K, Cc, _stream()), what)
     return y
 
 
@@ -1418,9 +1435,9 @@ def token_combine_backward(dy, ys, plan: TokenPlan, w):
         raise ValueError(f"{what}: dy has {Cd} channels, ys {Cc}")
     _fp32_vec(w, (T, K), what, "w")
     use_format(ys.dtype)
-    dys = torch.empty((T * K, Cc), dtype=ys.dtype, device=ys.device)
-    dw = torch.empty((T, K), dtype=torch.float32, device=ys.device)
-    check(lib.ymk_token_combine_backward(DT[ys.dtype], _p(dy), lddy, _p(ys), ldys, _p(plan.row), _p(w), _p(dys), Cc, _p(dw), T, K, Cc, _stream()), what)
+    dys, dw = ys.new_empty(T * K, Cc), torch.empty_like(w)
+    check(lib.ymk_token_combine_backward(DT[ys.dtype], dy.data_ptr(), lddy, ys.data_ptr(), ldys, plan.row.data_ptr(), w.data_ptr(), dys.data_ptr(), Cc, dw.data_ptr(),
+                                         T, K, Cc, _stream()), what)
     return dys, dw
 
 
@@ -1430,7 +1447,7 @@ def _expert_args(what, x, w, offsets):
     if w.dim() != 3 or not w.is_contiguous() or 0 in w.shape:
         raise ValueError(f"{what}: w is a contiguous [experts, Cout, Cin] tensor, got {list(w.shape)}")
     E, Cout, Cin = w.shape
-    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (E + 1,) or not offsets.is_contiguous():
+    if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or not offsets.is_contiguous():
         raise ValueError(f"{what}: offsets is a contiguous int32 [{E + 1}] tensor")
     if E > _lib.TOKEN_MAX_E:
         raise ValueError(f"{what}: {E} experts (at most {_lib.TOKEN_MAX_E})")
@@ -1476,9 +1493,9 @@ def expert_linear(x, w, offsets, bias=None, act=None, x_scale=None, w_scale=None
         _fp32_vec(bias, (E, Cout), what, "bias")
     if act not in _ROW_ACT:
         raise ValueError(f"{what}: act {act!r}")
-    y = torch.empty((M, Cout), dtype=odt, device=x.device)
-    check(lib.ymk_expert_linear(_ROW_DT[x.dtype], DT[odt], _p(x), ldx, _p(x_scale), _p(w), _p(w_scale), _p(bias), _p(offsets), _p(y), Cout, M, E, Cin, Cout,
-                                _ROW_ACT[act], _stream()), what)
+    y = x.new_empty((M, Cout), dtype=odt)
+    check(lib.ymk_expert_linear(_ROW_DT[x.dtype], DT[odt], x.data_ptr(), ldx, _ptr(x_scale), w.data_ptr(), _ptr(w_scale), _ptr(bias), offsets.data_ptr(), y.data_ptr(),
+                                Cout, M, E, Cin, Cout, _ROW_ACT[act], _stream()), what)
     return y
 
 
@@ -1501,11 +1518,12 @@ def expert_linear_backward(dy, x, w, offsets, need_dx: bool = True, need_dw: boo
         raise ValueError(f"{what}: {M} rows of x, {Md} of dy, or w is not 16-byte aligned")
     dx = dw = db = None
     if need_dx:
-        dx = torch.empty((M, Cin), dtype=x.dtype, device=x.device)
-        check(lib.ymk_expert_linear_dx(DT[x.dtype], _p(dy), lddy, _p(w), _p(offsets), _p(dx), Cin, M, E, Cin, Cout, _stream()), "expert_linear_dx")
+        dx = x.new_empty(M, Cin)
+        check(lib.ymk_expert_linear_dx(DT[x.dtype], dy.data_ptr(), lddy, w.data_ptr(), offsets.data_ptr(), dx.data_ptr(), Cin, M, E, Cin, Cout, _stream()),
+              "expert_linear_dx")
     if need_dw:
-        dw = torch.empty((E, Cout, Cin), dtype=dw_dtype or x.dtype, device=x.device)
-        db = torch.empty((E, Cout), dtype=torch.float32, device=x.device) if need_db else None
-        check(lib.ymk_expert_linear_dw(DT[x.dtype], DT[dw.dtype], _p(dy), lddy, _p(x), ldx, _p(offsets), _p(dw), _p(db), M, E, Cin, Cout, _stream()),
-              "expert_linear_dw")
+        dw = torch.empty_like(w, dtype=dw_dtype or x.dtype)
+        db = x.new_empty((E, Cout), dtype=torch.float32) if need_db else None
+        check(lib.ymk_expert_linear_dw(DT[x.dtype], DT[dw.dtype], dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(), dw.data_ptr(), _ptr(db), M, E, Cin, Cout,
+                                       _stream()), "expert_linear_dw")
     return dx, dw, db
