@@ -53,7 +53,7 @@ def build(force: bool = False, f16: bool = False) -> Path | None:
 def _build_locked(cxx, force: bool, f16: bool) -> Path:
     lib = OUT / ("libymk_hostemu_f16.so" if f16 else "libymk_hostemu.so")
     srcs = [CSRC / s for s in SOURCES]
-    deps = srcs + [CSRC / "ymk_common.h", CSRC / "glds.h", CSRC / "igemm.h", ROOT / "include" / "ymk_mixture.h", ROOT / "include" / "ymk_tokens.h", HERE / "hip" / "hip_runtime.h", Path(__file__)]
+    deps = srcs + [CSRC / "ymk_common.h", CSRC / "glds.h", CSRC / "igemm.h", CSRC / "rows.h", ROOT / "include" / "ymk_mixture.h", ROOT / "include" / "ymk_tokens.h", HERE / "hip" / "hip_runtime.h", Path(__file__)]
     if not force and lib.exists() and lib.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
         return lib
     units = []
@@ -64,6 +64,7 @@ def _build_locked(cxx, force: bool, f16: bool) -> Path:
         txt = re.sub(r"\b__shared__\b", "static", txt)
         txt = txt.replace('#include "ymk_common.h"', f'#include "{CSRC / "ymk_common.h"}"')
         txt = txt.replace('#include "igemm.h"', f'#include "{CSRC / "igemm.h"}"')
+        txt = txt.replace('#include "rows.h"', f'#include "{CSRC / "rows.h"}"')
         txt = txt.replace('#include "glds.h"', f'#include "{CSRC / "glds.h"}"')
         txt = txt.replace('#include "../../include/ymk_mixture.h"', f'#include "{ROOT / "include" / "ymk_mixture.h"}"')
         txt = txt.replace('#include "../../include/ymk_tokens.h"', f'#include "{ROOT / "include" / "ymk_tokens.h"}"')

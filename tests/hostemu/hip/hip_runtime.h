@@ -321,6 +321,24 @@ static inline hostemu_f32x16 __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(hos
     }
     return hostemu::mfma32(32, c);
 }
+static inline hostemu_f32x4 __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(hostemu_i32x8 a, hostemu_i32x8 b, hostemu_f32x4 c, int fmt_a, int fmt_b, int, int, int, int) {
+    if (fmt_a || fmt_b) abort();   // e4m3 only
+    const unsigned t = hostemu::cur, w0 = t & ~63u, l = t & 63u;
+    for (int e = 0; e < 32; ++e) {
+        hostemu::mfma_wide_a[t][e] = hostemu::from_e4m3(((unsigned)a[e / 4] >> (e % 4 * 8)) & 255u);
+        hostemu::mfma_wide_b[t][e] = hostemu::from_e4m3(((unsigned)b[e / 4] >> (e % 4 * 8)) & 255u);
+    }
+    hostemu::wave_sync();
+    for (int r = 0; r < 4; ++r) {
+        const unsigned i = (l / 16) * 4 + r, j = l % 16;
+        float s = 0.f;
+        for (unsigned h = 0; h < 4; ++h)
+            for (int e = 0; e < 32; ++e) s += hostemu::mfma_wide_a[w0 + h * 16 + i][e] * hostemu::mfma_wide_b[w0 + h * 16 + j][e];
+        c[r] += s;
+    }
+    hostemu::wave_sync();
+    return c;
+}
 static inline int __builtin_amdgcn_cvt_pk_fp8_f32(float x, float y, int old, bool high) {
     const unsigned v = hostemu::to_e4m3(x) | (hostemu::to_e4m3(y) << 8);
     return (int)(high ? ((unsigned)old & 0xffffu) | (v << 16) : ((unsigned)old & 0xffff0000u) | v);

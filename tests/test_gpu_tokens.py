@@ -1,5 +1,10 @@
 """The token operators (include/ymk_tokens.h) on the GPU: the checks of tests/token_cases.py that the lane emulator runs too, the sizes it is too slow
 for, and what only the hardware shows — captured graphs, side streams, the same bits on every run."""
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -86,6 +91,21 @@ def test_product_gradient(ops, dtype, case):
 def test_product_gradient_in_32_bits(ops):
     tc.check_product_gradient(ops, torch.bfloat16, ([40, 3], 0, 24, 40, None, 8), DEV, dw_dtype=torch.float32)
     tc.check_product_gradient(ops, torch.bfloat16, ([1400, 0, 300], 0, 256, 320, None, 0), DEV, dw_dtype=torch.float32)
+
+
+@pytest.mark.parametrize("tile", ["16", "64", "128", "256"])
+def test_product_at_every_tile(tile):
+    """Each tile of the product on sizes that the rule would give to another (the switch is read once a process)."""
+    code = (
+        "import torch\n"
+        "from tests import token_cases as tc, test_gpu_tokens as t\n"
+        "from yolo_master_amd import ops\n"
+        "for c in tc.PRODUCTS + t.BIG:\n"
+        "    for d in t.DTYPES: tc.check_product(ops, d, c, t.DEV); tc.check_product_gradient(ops, d, c, t.DEV)\n"
+        "    if c[2] % 16 == 0: tc.check_product_exact(ops, c, t.DEV)\n"
+        "tc.check_product_gradient(ops, torch.bfloat16, t.BIG[0], t.DEV, dw_dtype=torch.float32)\n"
+        "tc.check_product(ops, t.E4M3, t.BIG[1], t.DEV, out_dtype=torch.float32)\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=str(Path(__file__).resolve().parent.parent), env={**os.environ, "YMK_EXPERT_TILE": tile}, timeout=110)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

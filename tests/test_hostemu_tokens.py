@@ -1,6 +1,10 @@
 """The token operators (csrc/rmsnorm.hip, tokens.hip, expert.hip; include/ymk_tokens.h) on the CPU lane emulator, through the product's own wrappers:
 every check of tests/token_cases.py, the refusals of the wrappers and of the C entry points, and the header against its ctypes table."""
 import ctypes as C
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -100,6 +104,24 @@ def test_product_gradient(ops, dtype, case):
 
 def test_product_gradient_in_32_bits(ops):
     tc.check_product_gradient(ops, torch.bfloat16, ([40, 3], 0, 24, 40, None, 8), dw_dtype=torch.float32)
+
+
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
+def test_product_at_every_tile(tile, libs):
+    """Each tile on sizes that the rule would give to another (the switch is read once a process)."""
+    code = (
+        "import torch, ctypes as C\n"
+        "from tests import token_cases as tc\n"
+        "from tests.hostemu import build\n"
+        "from yolo_master_amd import _lib, ops\n"
+        "h = C.CDLL(str(build.build()))\n"
+        "for name, (res, args) in _lib.SYMBOLS_TOKENS.items(): fn = getattr(h, name); fn.restype, fn.argtypes = res, args\n"
+        "ops.lib, ops._stream, ops.require_gpu = h, lambda: None, lambda t, what='': None\n"
+        "for c in (([130, 0, 1, 37], 3, 80, 144, 'gelu', 0), ([5, 129], 0, 208, 16, 'sigmoid', 0)):\n"
+        "    for d in (torch.float32, torch.bfloat16): tc.check_product(ops, d, c); tc.check_product_gradient(ops, d, c)\n"
+        "    tc.check_product_exact(ops, c)\n"
+        "    tc.check_product(ops, torch.float8_e4m3fn, c, out_dtype=torch.float32)\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=str(Path(__file__).resolve().parent.parent), env={**os.environ, "YMK_EXPERT_TILE": tile}, timeout=600)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

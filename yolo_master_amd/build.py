@@ -30,7 +30,7 @@ SOURCES = ["capi.hip", "conv.hip", "dwconv.hip", "mlp.hip", "stem2.hip", "c3k2f.
            "mixture.hip", "mixattn.hip",   # config-5 rows, first implementation (include/ymk_mixture.h)
            *TOKEN_SOURCES,
            "conv_glds.hip", "post.hip", "preproc.hip"]   # LDS-DMA tiled convolution core, box rescaling / validation matching, letterbox (include/ymk_next.h)
-HEADERS = ["ymk_common.h", "igemm.h", "glds.h", "../../include/ymk.h", "../../include/ymk_mixture.h", "../../include/ymk_next.h", "../../include/ymk_tokens.h"]
+HEADERS = ["ymk_common.h", "igemm.h", "glds.h", "rows.h", "../../include/ymk.h", "../../include/ymk_mixture.h", "../../include/ymk_next.h", "../../include/ymk_tokens.h"]
 
 
 def _hipcc() -> str:

@@ -139,13 +139,16 @@ __device__ __forceinline__ int ex_perm(int i) { return ((i >> 2) & 1) * 16 + (i 
 // `spread`: rows permuted (the N side; the transposing reader permutes its columns by itself, for either side).
 //   KC:  row r at r * 128, its 16-byte piece c in slot c ^ ((r >> 1) & 7): the 16 rows that a 16-byte read serves at once (0-3, 12-15, 20-23, 24-27 and
 //        their complement, or 16 in a row) cover all 64 banks
-//   !KC: k-row k at k * TILE * ES; 16-bit pieces c in slot c ^ ((k & 3) << 2): the four k-rows by 64 bytes that half a wave's transposing read takes do
+//   !KC: k-row k at k * TILE * ES; 16-bit pieces c in slot c ^ ((k & 3) << 2), in rows of 128 bytes c ^ (k & 2) << 1: the four k-rows by 64 bytes that half
+//        a wave's transposing read takes do
 template <typename T, bool KC, int TILE>
 struct ExSide {
     static constexpr int ES = ExElem<T>::ES, KS = 128 / ES;   // elements of K a step
     static constexpr int LPR = KC ? 8 : TILE * ES / 16;        // lanes (16-byte pieces) of an LDS row
     static constexpr int RPI = 64 / LPR;                       // rows a wave brings with one transfer (TILE * ES <= 1024)
     static constexpr int LOADS = TILE / 32;                    // transfers of a wave a step
+
+    static __device__ __forceinline__ int swizzle(int k) { return TILE >= 128 ? (k & 3) << 2 : (k & 2) << 1; }
 
     const char* base;
     unsigned voff[LOADS];
@@ -171,7 +174,7 @@ struct ExSide {
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
                 const int k = (j * 4 + wave) * RPI + lr;
-                const int sc = ES == 2 ? pc ^ ((k & 3) << 2) : pc;
+                const int sc = ES == 2 ? pc ^ swizzle(k) : pc;
                 kfirst[j] = k;
                 voff[j] = first + sc * (16 / ES) < limit ? (unsigned)(k * ld + sc * 16) : 0x80000000u;
             }
@@ -199,7 +202,7 @@ struct ExSide {
             // elements of the permuted columns 4 * (lane % 4) .. + 3 of this half of the block
             const int i = lane & 15, g = (lane >> 4) & 1, h = lane >> 5, q = i & 3, kk = i >> 2;
             const int col = r0 + (q & 1) * 16 + (2 * g + (q >> 1)) * 4;
-            const int slot = (col >> 3) ^ (kk << 2);
+            const int slot = (col >> 3) ^ swizzle(kk);
             const char* p = src + (half * 32 + h * 8 + kk) * (TILE * 2) + slot * 16 + (col & 4) * 2;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -220,10 +223,10 @@ struct ExSide {
 // The tile of a workgroup among all experts' tiles, from the offsets alone (the host does not know them).  Workgroups b, b + 8, ... run on one XCD:
 // each XCD takes a contiguous range of tiles, and within it GM tiles of rows against all tiles of channels before the next GM.
 struct ExTile { int e, m0, mend, n0; };
-template <int TILE>
+template <int TM, int TN>
 __device__ __forceinline__ bool ex_find(const ExArgs& a, ExTile& t) {
     constexpr int GM = 8, CH = YMK_TOKEN_MAX_E / 64;
-    const int lane = threadIdx.x & 63, nt = (a.N + TILE - 1) / TILE;
+    const int lane = threadIdx.x & 63, nt = (a.N + TN - 1) / TN;
     int incl[CH], first[CH], last[CH], total = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -233,7 +236,7 @@ __device__ __forceinline__ bool ex_find(const ExArgs& a, ExTile& t) {
             first[c] = min(max(a.offsets[e], 0), a.rows);
             last[c] = min(max(a.offsets[e + 1], first[c]), a.rows);
         }
-        int s = (last[c] - first[c] + TILE - 1) / TILE;
+        int s = (last[c] - first[c] + TM - 1) / TM;
         for (int o = 1; o < 64; o <<= 1) {
             const int v = __shfl_up(s, o);
             if (lane >= o) s += v;
@@ -244,7 +247,7 @@ __device__ __forceinline__ bool ex_find(const ExArgs& a, ExTile& t) {
     const int all = total * nt, per = (all + 7) / 8, slot = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + slot;
     if (slot >= per || id >= all) return false;
     const int g = id / (GM * nt), size = min(GM, total - g * GM), r = id - g * (GM * nt), m = g * GM + r % size;
-    t.n0 = r / size * TILE;
+    t.n0 = r / size * TN;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const unsigned long long past = __ballot(incl[c] > m);   // the first of them is the expert
@@ -253,8 +256,8 @@ __device__ __forceinline__ bool ex_find(const ExArgs& a, ExTile& t) {
             t.e = c * 64 + l;
             const int f = __builtin_amdgcn_readlane(first[c], l);
             t.mend = __builtin_amdgcn_readlane(last[c], l);
-            const int tiles = (t.mend - f + TILE - 1) / TILE;
-            t.m0 = f + (m - (__builtin_amdgcn_readlane(incl[c], l) - tiles)) * TILE;
+            const int tiles = (t.mend - f + TM - 1) / TM;
+            t.m0 = f + (m - (__builtin_amdgcn_readlane(incl[c], l) - tiles)) * TM;
             return true;
         }
     }
@@ -448,15 +451,128 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
 
 // y and dx
 template <typename T, typename TO, bool NKC, int TILE>
-__global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void expert_rows_kernel(ExArgs a) {
+__global__ __launch_bounds__(256, TILE == 256 ? 1 : TILE == 128 ? 2 : 4) void expert_rows_kernel(ExArgs a) {
     ExTile t;
-    if (!ex_find<TILE>(a, t)) return;
+    if (!ex_find<TILE, TILE>(a, t)) return;
     ex_body<T, TO, NKC, true, TILE, false>(a, t, a.K, a.n + t.e * a.n_expert, a.m);
+}
+
+// y for few rows an expert: bound by the bytes of the experts' matrices.  A workgroup takes 16 rows by 32 channels; its four waves take the 128-byte pieces
+// of K in turn, EX_FEW_AHEAD of them in flight, straight from memory into the operands of the 16 x 16 matrix instructions (no LDS: nothing of W is used
+// twice), and add their sums up through LDS in the order of the waves.
+#define EX_FEW_N 32
+#define EX_FEW_AHEAD 4
+template <typename T>
+__device__ __forceinline__ f32x4 ex_mfma16(const ExFrag& a, const ExFrag& b, f32x4 c) {
+    if constexpr (std::is_same<T, E4m3>::value) {
+        i32x8 x, y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = (int)a.p[0][i]; x[4 + i] = (int)a.p[1][i];
+            y[i] = (int)b.p[0][i]; y[4 + i] = (int)b.p[1][i];
+        }
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = a.p[q][e], y = b.p[q][e];
+                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x), __uint_as_float(y), c, 0, 0, 0);
+                }
+            } else c = mfma16x16x32_h16(a.p[q], b.p[q], c);
+        }
+        return c;
+    }
+}
+
+template <typename T, typename TO>
+__global__ __launch_bounds__(256) void expert_few_rows_kernel(ExArgs a) {
+    constexpr int ES = ExElem<T>::ES, NB = EX_FEW_N / 16;
+    __shared__ float part[4][16][EX_FEW_N + 1];   // [wave][row][channel]
+    ExTile t;
+    if (!ex_find<16, EX_FEW_N>(a, t)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, piece = (lane >> 4) * 16;
+    // rows and channels behind the last one repeat it: their results are not stored
+    const char* xp = a.m + (int64_t)min(t.m0 + r, t.mend - 1) * a.m_ld;
+    const char* wp[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) wp[i] = a.n + t.e * a.n_expert + (int64_t)min(t.n0 + i * 16 + r, a.N - 1) * a.n_ld;
+    const int bytes = a.K * ES, full = bytes >> 7;   // whole pieces of K; the rest is less than one
+    f32x4 acc[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto load = [&](const char* p, int at) {
+        ExFrag f;
+        f.p[0] = *reinterpret_cast<const u32x4*>(p + at + piece);
+        f.p[1] = *reinterpret_cast<const u32x4*>(p + at + 64 + piece);
+        return f;
+    };
+    int k = wave;
+    for (; k + 4 * (EX_FEW_AHEAD - 1) < full; k += 4 * EX_FEW_AHEAD) {
+        ExFrag x[EX_FEW_AHEAD], w[EX_FEW_AHEAD][NB];
+#pragma unroll
+        for (int u = 0; u < EX_FEW_AHEAD; ++u) {
+            x[u] = load(xp, (k + 4 * u) * 128);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) w[u][i] = load(wp[i], (k + 4 * u) * 128);
+        }
+        EX_SCHED_FENCE();   // all of them are on their way before the first is waited for
+#pragma unroll
+        for (int u = 0; u < EX_FEW_AHEAD; ++u)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) acc[i] = ex_mfma16<T>(w[u][i], x[u], acc[i]);
+    }
+    for (; k < full; k += 4) {
+        const ExFrag x = load(xp, k * 128);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] = ex_mfma16<T>(load(wp[i], k * 128), x, acc[i]);
+    }
+    if (k == full && (bytes & 127)) {   // the last piece: 16-byte parts behind K are zeros on both sides
+        auto tail = [&](const char* p) {
+            ExFrag f;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int at = full * 128 + q * 64 + piece;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(p + (at < bytes ? at : 0));
+                f.p[q] = at < bytes ? v : u32x4{0, 0, 0, 0};
+            }
+            return f;
+        };
+        const ExFrag x = tail(xp);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] = ex_mfma16<T>(tail(wp[i]), x, acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) part[wave][r][i * 16 + (lane >> 4) * 4 + q] = acc[i][q];
+    __syncthreads();
+    const int row = t.m0 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 2;   // two channels of a row a thread
+    if (row >= t.mend || t.n0 + c >= a.N) return;                            // N is even
+    const float ms = a.m_scale ? a.m_scale[row] : 1.f;
+    float v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const float(*p)[16][EX_FEW_N + 1] = part;
+        const int q = threadIdx.x >> 4;
+        v[e] = (p[0][q][c + e] + p[1][q][c + e]) + (p[2][q][c + e] + p[3][q][c + e]);
+        const int64_t at = (int64_t)t.e * a.N + t.n0 + c + e;
+        if (a.n_scale) v[e] *= ms * a.n_scale[at];
+        if (a.bias) v[e] += a.bias[at];
+        if (a.act == YMK_ACT_SILU) v[e] = ex_act<YMK_ACT_SILU, sizeof(TO) == 2>(v[e]);
+        else if (a.act == YMK_ACT_GELU) v[e] = ex_act<YMK_ACT_GELU, sizeof(TO) == 2>(v[e]);
+        else if (a.act == YMK_ACT_SIGMOID) v[e] = ex_act<YMK_ACT_SIGMOID, sizeof(TO) == 2>(v[e]);
+    }
+    TO* out = reinterpret_cast<TO*>(a.out) + (int64_t)row * a.out_ld + t.n0 + c;
+    if constexpr (sizeof(TO) == 4) *reinterpret_cast<f32x2*>(out) = f32x2{v[0], v[1]};
+    else *reinterpret_cast<uint32_t*>(out) = pack_h16x2(v[0], v[1]);
 }
 
 // dW (and, by the workgroups of the first channels, db)
 template <typename T, typename TO, int TILE>
-__global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void expert_dw_kernel(ExArgs a) {
+__global__ __launch_bounds__(256, TILE == 256 ? 1 : TILE == 128 ? 2 : 4) void expert_dw_kernel(ExArgs a) {
     // Experts differ in rows, so each expert's tiles are split over all XCDs: eight runs of neighbouring tiles, one an XCD (32768 rows over 8 experts
     // drawn with a spread of 0.3, 1024 by 4096: an expert an XCD took 324 us, this 278 us); fewer than eight tiles go round in turn.
     const int nt = (a.N + TILE - 1) / TILE, mt = (a.M + TILE - 1) / TILE, all = nt * mt, run = (all + 7) / 8;
@@ -489,20 +605,56 @@ int ex_launch(const ExArgs& a, int64_t blocks, size_t lds, void* stream) {
 }
 
 // workgroups that hold every tile of rows whatever the offsets say, in whole rounds of the 8 XCDs
-inline int64_t ex_blocks(int64_t rows, int E, int N, int tile) {
-    const int64_t mt = rows / tile + (rows < E ? rows : E), nt = (N + tile - 1) / tile;
+inline int64_t ex_blocks(int64_t rows, int E, int N, int tm, int tn) {
+    const int64_t mt = rows / tm + (rows < E ? rows : E), nt = (N + tn - 1) / tn;
     return (mt * nt + 7) / 8 * 8;
 }
 
-// Tiles of 256 halve the bytes that reach LDS for a product, but leave CUs idle when there are few and waste rows when experts have few
-// (bf16, 32768 rows 4096 -> 4096 over 8 experts: 1009 us against 1159; 4096 rows 512 -> 2048 over 16: 22.8 against 24.6; e4m3, 4096 rows 1024 -> 2048
-// over 32: 40.2 against 28.1): from 192 rows an expert and one tile a CU on.
-inline bool ex_wide(int64_t rows, int E, int N) { return rows >= 192ll * E && (rows / 256 + E / 2) * ((N + 255) / 256) >= 256; }
+// Wider tiles bring fewer bytes to LDS for a product, but leave CUs idle when there are few of them and waste rows when experts have few.  Both sides, us:
+//     rows an expert   shape (16-bit unless said)              16     64    128    256
+//     1                6 rows of 64 experts, 4096 -> 2048 e4m3  9.4   12.9   16.9   39.6
+//     2                16 of 8, 2048 -> 4096                   24.1   23.2   24.0   46.7
+//     16               128 of 8, 2048 -> 4096                  36.6   24.3   25.4   44.6
+//     64               512 of 8, 2048 -> 4096                 100.5   31.9   28.5   47.4
+//     64               1024 of 16, 1024 -> 2048                60.2   16.3   16.7   27.9
+//     200              3202 of 16, 256 -> 520 fp32             31.3   18.9   23.9   70.3
+//     256              4096 of 16, 512 -> 2048                123.8   26.1   22.3   22.8
+//     4096             32768 of 8, 4096 -> 4096                              1159   1009
+inline int ex_tile(int64_t rows, int E, int N) {
+    auto tiles = [&](int tile) { return (rows / tile + E / 2) * ((N + tile - 1) / tile); };
+    if (rows <= 16 || rows <= 4ll * E) return 16;
+    if (rows >= 192ll * E && tiles(256) >= 256) return 256;
+    if (rows >= 32ll * E && tiles(128) >= 256) return 128;
+    return 64;
+}
 
+// A/B and test switch, read at first use: YMK_EXPERT_TILE=16|64|128|256 takes that tile for every size (16: y only; the others then take 64)
+inline int ex_forced() {
+    static const int tile = [] {
+        const char* s = getenv("YMK_EXPERT_TILE");
+        const int v = s ? atoi(s) : 0;
+        return v == 16 || v == 64 || v == 128 || v == 256 ? v : 0;
+    }();
+    return tile;
+}
+template <typename T, typename TO, bool NKC, int TILE>
+int ex_rows_tile(const ExArgs& a, void* stream) {
+    return ex_launch<expert_rows_kernel<T, TO, NKC, TILE>>(a, ex_blocks(a.rows, a.E, a.N, TILE, TILE), EX_UNITS * TILE * 128, stream);
+}
 template <typename T, typename TO, bool NKC>
 int ex_rows(const ExArgs& a, void* stream) {
-    if (ex_wide(a.rows, a.E, a.N)) return ex_launch<expert_rows_kernel<T, TO, NKC, 256>>(a, ex_blocks(a.rows, a.E, a.N, 256), EX_UNITS * 256 * 128, stream);
-    return ex_launch<expert_rows_kernel<T, TO, NKC, 128>>(a, ex_blocks(a.rows, a.E, a.N, 128), EX_UNITS * 128 * 128, stream);
+    const int tile = ex_forced() ? ex_forced() : ex_tile(a.rows, a.E, a.N);
+    if constexpr (NKC) {
+        if (tile == 16) {
+            const int64_t blocks = ex_blocks(a.rows, a.E, a.N, 16, EX_FEW_N);
+            if (blocks > 0x7fffffff) return YMK_E_BADARG;
+            hipLaunchKernelGGL((expert_few_rows_kernel<T, TO>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+            return ymk_launch_status();
+        }
+    }
+    if (tile == 256) return ex_rows_tile<T, TO, NKC, 256>(a, stream);
+    if (tile == 128) return ex_rows_tile<T, TO, NKC, 128>(a, stream);
+    return ex_rows_tile<T, TO, NKC, 64>(a, stream);
 }
 inline int64_t ex_dw_blocks(const ExArgs& a, int tile) {
     const int64_t all = (int64_t)((a.N + tile - 1) / tile) * ((a.M + tile - 1) / tile);
@@ -510,8 +662,12 @@ inline int64_t ex_dw_blocks(const ExArgs& a, int tile) {
 }
 template <typename T, typename TO>
 int ex_dw(const ExArgs& a, void* stream) {
-    if (ex_dw_blocks(a, 256) >= 512) return ex_launch<expert_dw_kernel<T, TO, 256>>(a, ex_dw_blocks(a, 256), EX_UNITS * 256 * 128, stream);
-    return ex_launch<expert_dw_kernel<T, TO, 128>>(a, ex_dw_blocks(a, 128), EX_UNITS * 128 * 128, stream);
+    // us at 64 / 128 / 256: 200 rows an expert, 16 of 520 x 256 fp32 18.9 / 31.0 / 88; 64 rows, 16 of 2048 x 1024 30.6 / 24.6 / 26.9; 256 rows, 16 of
+    // 2048 x 512 26.0 / 22.4 / 25.3; 4096 rows, 8 of 4096 x 1024 - / 353 / 318
+    const int tile = ex_forced() ? ex_forced() : a.rows >= 1024ll * a.E && ex_dw_blocks(a, 256) >= 512 ? 256 : ex_dw_blocks(a, 128) >= 512 ? 128 : 64;
+    if (tile == 256) return ex_launch<expert_dw_kernel<T, TO, 256>>(a, ex_dw_blocks(a, 256), EX_UNITS * 256 * 128, stream);
+    if (tile == 128) return ex_launch<expert_dw_kernel<T, TO, 128>>(a, ex_dw_blocks(a, 128), EX_UNITS * 128 * 128, stream);
+    return ex_launch<expert_dw_kernel<T, TO, 64>>(a, ex_dw_blocks(a, 64), EX_UNITS * 64 * 128, stream);
 }
 
 inline bool ex_bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15); }

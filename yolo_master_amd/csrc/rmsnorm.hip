@@ -2,53 +2,56 @@
 //
 // Memory-bound: a row is read once, kept in registers between the statistic and the output, and written once.  A row belongs to a group of
 // 2^n lanes (8..64 of one wave, or a whole workgroup of 128..1024): a lane holds up to NV vectors of V elements, vector i of lane l at column
-// (l + i * group) * V, so every load and store of a group is contiguous.  V is 16 bytes where rows are 16-byte aligned and single elements
-// otherwise.  Groups of one wave need no LDS and no barrier, so they take every width that fits their registers once there are rows enough;
+// (l + i * group) * V, so every load and store of a group is contiguous; V is 16 bytes (csrc/rows.h).  Groups of one wave need no LDS and no barrier, so they take every width that fits their registers once there are rows enough;
 // wide rows, and few rows, are spread over a workgroup.
 #include "ymk_common.h"
+#include "rows.h"
 #include "../../include/ymk_tokens.h"
 
 #ifndef YMK_MAX_BLOCKS
 #define RN_MAX_WAVES (256 * 32)   // waves of the one-wave kernels that stay resident and walk the rows: 8 per SIMD
 #define RN_MAX_GROUPS 2048        // ... and workgroups of the wide ones
-#define RN_BWD_BLOCKS 1024        // workgroups of the gradient: each leaves one partial row of dweight
+#define RN_BWD_BLOCKS 1280        // workgroups of the gradient: each leaves one partial row of dweight
 #else
 #define RN_MAX_WAVES 8
 #define RN_MAX_GROUPS YMK_MAX_BLOCKS
 #define RN_BWD_BLOCKS YMK_MAX_BLOCKS
 #endif
 
+#define RN_MAX_NV(T) (2 * (int)sizeof(T))    // vectors a lane holds at most: 32 values,
+#define RN_MAX_NV_BWD(T) ((int)sizeof(T))    // 16 in the gradient, which keeps five of each (128 registers)
 #define RN_TINY 0x1.cp-118f   // 448 * 2^-126: below it the scale would be subnormal and its reciprocal infinite
 
 namespace {
 
-template <typename T, int V>
-__device__ __forceinline__ void rn_load(const T* p, float (&v)[V]) {
-    if constexpr (V == 1) v[0] = to_f32(*p);
-    else load_vec_f32(p, v);
-}
-template <typename T, int V>
-__device__ __forceinline__ void rn_store(T* p, const float (&v)[V]) {
-    if constexpr (V == 1) from_f32(*p, v[0]);
-    else store_vec_f32(p, v);
-}
 // the value as it is stored
 template <typename T>
 __device__ __forceinline__ float rn_round(float v) {
     if constexpr (sizeof(T) == 4) return v;
     else return h16_to_f32(f32_to_h16(v));
 }
-__device__ __forceinline__ void rn_store_e4m3(uint8_t* p, const float (&v)[8]) {
-    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
-    *reinterpret_cast<u32x2*>(p) = u32x2{(uint32_t)lo, (uint32_t)hi};
+// the first n of V values in e4m3
+__device__ __forceinline__ uint32_t rn_e4m3(float a, float b, float c, float d) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
-__device__ __forceinline__ void rn_store_e4m3(uint8_t* p, const float (&v)[4]) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-    *reinterpret_cast<uint32_t*>(p) = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+template <bool EVEN, int V>
+__device__ __forceinline__ void rn_store_e4m3(uint8_t* p, int n, const float (&v)[V]) {
+    if (EVEN || n >= V) {
+        if constexpr (V == 8) {
+            const u32x2 w{rn_e4m3(v[0], v[1], v[2], v[3]), rn_e4m3(v[4], v[5], v[6], v[7])};
+            if constexpr (EVEN) *reinterpret_cast<u32x2*>(p) = w;
+            else *reinterpret_cast<u32x2_u*>(p) = w;
+        } else {
+            const uint32_t w = rn_e4m3(v[0], v[1], v[2], v[3]);
+            if constexpr (EVEN) *reinterpret_cast<uint32_t*>(p) = w;
+            else *reinterpret_cast<u32_u*>(p) = w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V - 1; ++e)
+            if (e < n) p[e] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[e], 0.f, 0, false);
+    }
 }
-__device__ __forceinline__ void rn_store_e4m3(uint8_t* p, const float (&v)[1]) { *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0], 0.f, 0, false); }
 
 // Sum (and, below, largest bit pattern) over the group of a lane: lanes [l - l % group, + group) of a wave, or all `group` lanes of the workgroup
 // through LDS (two slots used in turn: one barrier a reduction).  Every lane gets the result of the same tree: bit-identical within the group.
@@ -86,8 +89,9 @@ struct RnArgs {
     float eps;
 };
 
-template <typename T, int V, int NV, bool QUANT>
+template <typename T, bool EVEN, int NV, bool QUANT>
 __global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
+    constexpr int V = 16 / sizeof(T);
     __shared__ float part[2][16];
     RnGroup g{a.group, 0, part};
     const int lane = threadIdx.x & (a.group - 1), per = blockDim.x / a.group;
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
     for (int i = 0; i < NV; ++i) {
         const int c = (lane + i * a.group) * V;
 #pragma unroll
-        for (int e = 0; e < V; ++e) w[i][e] = c < a.C ? a.weight[c + e] : 0.f;
+        for (int e = 0; e < V; ++e) w[i][e] = c + e < a.C ? a.weight[c + e] : 0.f;
     }
     const float inv_c = 1.0f / (float)a.C;
     for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < a.rows; r0 += (int64_t)gridDim.x * per) {   // the same trips for the whole workgroup
@@ -111,7 +115,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
             const int c = (lane + i * a.group) * V;
 #pragma unroll
             for (int e = 0; e < V; ++e) v[i][e] = 0.f;
-            if (c < cols) rn_load<T, V>(x + r * a.ldx + c, v[i]);
+            if (c < cols) row_load<T, EVEN>(x + r * a.ldx + c, cols - c, v[i]);
         }
         if (res) {
 #pragma unroll
@@ -119,7 +123,9 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
                 const int c = (lane + i * a.group) * V;
                 if (c < cols) {
                     float b[V];
-                    rn_load<T, V>(res + r * a.ldr + c, b);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) b[e] = 0.f;
+                    row_load<T, EVEN>(res + r * a.ldr + c, cols - c, b);
 #pragma unroll
                     for (int e = 0; e < V; ++e) v[i][e] = rn_round<T>(v[i][e] + b[e]);
                 }
@@ -134,7 +140,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (lane + i * a.group) * V;
-                if (c < cols) rn_store<T, V>(static_cast<T*>(a.h) + r * a.ldh + c, v[i]);
+                if (c < cols) row_store<T, EVEN>(static_cast<T*>(a.h) + r * a.ldh + c, cols - c, v[i]);
             }
         }
         float top = 0.f;
@@ -160,13 +166,13 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
                 const int c = (lane + i * a.group) * V;
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[i][e] = top < RN_TINY ? 0.f : v[i][e] * inv;
-                if (c < cols) rn_store_e4m3(static_cast<uint8_t*>(a.y) + r * a.ldy + c, v[i]);
+                if (c < cols) rn_store_e4m3<EVEN>(static_cast<uint8_t*>(a.y) + r * a.ldy + c, cols - c, v[i]);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (lane + i * a.group) * V;
-                if (c < cols) rn_store<T, V>(static_cast<T*>(a.y) + r * a.ldy + c, v[i]);
+                if (c < cols) row_store<T, EVEN>(static_cast<T*>(a.y) + r * a.ldy + c, cols - c, v[i]);
             }
         }
         if (a.stat && lane == 0 && cols) a.stat[r] = stat;
@@ -187,8 +193,9 @@ struct RnBwdArgs {
 
 // dx of a row in one pass over it; dweight: a lane sums its columns over the rows it walks, the groups of a workgroup are added in a fixed
 // order through LDS, and each workgroup leaves one partial row that rms_norm_dweight_kernel adds up — no atomics, the same bits every time.
-template <typename T, int V, int NV>
+template <typename T, bool EVEN, int NV>
 __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(RnBwdArgs a) {
+    constexpr int V = 16 / sizeof(T);
     __shared__ float part[2][16];
     extern __shared__ float dw_lds[];   // [groups of the workgroup][columns of a group]
     RnGroup g{a.group, 0, part};
@@ -202,7 +209,7 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(RnBwdArgs a) {
         const int c = (lane + i * a.group) * V;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            w[i][e] = c < a.C ? a.weight[c + e] : 0.f;
+            w[i][e] = c + e < a.C ? a.weight[c + e] : 0.f;
             dw[i][e] = 0.f;
         }
     }
@@ -218,9 +225,9 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(RnBwdArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) n[i][e] = d[i][e] = o[i][e] = 0.f;
             if (c < cols) {
-                rn_load<T, V>(hp + r * a.ldh + c, n[i]);
-                rn_load<T, V>(dyp + r * a.lddy + c, d[i]);
-                if (drp) rn_load<T, V>(drp + r * a.lddr + c, o[i]);
+                row_load<T, EVEN>(hp + r * a.ldh + c, cols - c, n[i]);
+                row_load<T, EVEN>(dyp + r * a.lddy + c, cols - c, d[i]);
+                if (drp) row_load<T, EVEN>(drp + r * a.lddr + c, cols - c, o[i]);
             }
         }
         float gn = 0.f;
@@ -239,7 +246,7 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(RnBwdArgs a) {
             const int c = (lane + i * a.group) * V;
 #pragma unroll
             for (int e = 0; e < V; ++e) o[i][e] = fmaf(rstd, fmaf(-n[i][e], gn, d[i][e]), o[i][e]);
-            if (c < cols) rn_store<T, V>(static_cast<T*>(a.dx) + r * a.lddx + c, o[i]);
+            if (c < cols) row_store<T, EVEN>(static_cast<T*>(a.dx) + r * a.lddx + c, cols - c, o[i]);
         }
     }
     if (!a.part) return;
@@ -250,7 +257,7 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(RnBwdArgs a) {
             const int c = (lane + i * a.group) * V;
 #pragma unroll
             for (int e = 0; e < V; ++e)
-                if (c < a.C) out[c + e] = dw[i][e];
+                if (c + e < a.C) out[c + e] = dw[i][e];
         }
         return;
     }
@@ -268,14 +275,26 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(RnBwdArgs a) {
     }
 }
 
-// dweight[c] = sum over the partial rows: 64 columns by 16 strands of rows a workgroup, added in strand order
+// dweight[c] = sum over the partial rows: 16 columns by 64 strands of rows a workgroup, four rows of a strand in flight at a time, added in strand order
+// (64 columns by 16 strands of one row at a time: 18 us for 915 partial rows of 256, all of it waiting)
 __global__ __launch_bounds__(1024) void rms_norm_dweight_kernel(const float* part, int blocks, int C, float* dweight) {
-    __shared__ float s[16][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+    __shared__ float s[64][17];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
     float v = 0.f;
     if (c < C)
-        for (int b = q; b < blocks; b += 16) v += part[(size_t)b * C + c];
-    s[q][threadIdx.x & 63] = v;
+        for (int b = q; b < blocks; b += 256) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = b + 64 * i < blocks ? part[(size_t)(b + 64 * i) * C + c] : 0.f;
+            v += (p[0] + p[1]) + (p[2] + p[3]);
+        }
+    s[q][threadIdx.x & 15] = v;
+    __syncthreads();
+    if (q < 16) {   // thread (strand group q, column)
+        v = (s[q][threadIdx.x & 15] + s[q + 16][threadIdx.x & 15]) + (s[q + 32][threadIdx.x & 15] + s[q + 48][threadIdx.x & 15]);
+        __syncthreads();
+        s[q][threadIdx.x & 15] = v;
+    } else __syncthreads();
     __syncthreads();
     if (q == 0 && c < C) {
         for (int i = 1; i < 16; ++i) v += s[i][threadIdx.x];
@@ -297,39 +316,46 @@ inline RnPlan rn_plan(int64_t rows, int32_t vecs, int max_nv, int64_t max_waves,
     const bool few = rows <= 512;
     p.group = 8;
     while (p.group < 64 && p.group * (few ? 1 : 2) < vecs) p.group *= 2;
-    while (p.group < 1024 && p.group * (few ? 1 : max_nv > 4 ? max_nv : 4) < vecs) p.group *= 2;
+    while (p.group < 1024 && p.group * (few ? 1 : max_nv) < vecs) p.group *= 2;
     p.nv = 1;
     while (p.group * p.nv < vecs) p.nv *= 2;
     p.threads = p.group > 64 ? p.group : 256;   // a group wider than a wave is a workgroup of its own
     const int per = p.threads / p.group;
     const int64_t need = (rows + per - 1) / per;                                        // workgroups if none walked
     const int64_t most = p.group > 64 ? max_groups : max_waves / (p.threads / 64);
-    const int64_t trips = (need + most - 1) / most;
-    p.grid = (unsigned)((need + trips - 1) / trips);                                    // equal trips for all
+    // Equal trips for all workgroups and an equal number of workgroups for all 256 CUs: of the next few trip counts the one whose fullest CU walks least
+    // (25600 rows of 2048, norm to 8 bits: 4 trips of 1600 workgroups, seven on some CUs, 97 us; 5 trips of 1280, five on each, 79 us)
+    int64_t trips = (need + most - 1) / most, walked = INT64_MAX;
+    for (int64_t t = trips, last = trips + 4; t < last; ++t) {
+        const int64_t grid = (need + t - 1) / t, w = t * ((grid + 255) / 256);
+        if (w < walked) {
+            walked = w;
+            trips = t;
+        }
+    }
+    p.grid = (unsigned)((need + trips - 1) / trips);
     return p;
 }
 
-template <typename T, int V, bool QUANT, int NV = 1>
+template <typename T, bool EVEN, bool QUANT, int NV = 1>
 int rn_launch(const RnPlan& p, const RnArgs& a, void* stream) {
-    if constexpr (NV > (V == 1 ? 16 : 4 * (int)sizeof(T) / 2)) return YMK_E_BADARG;
+    if constexpr (NV > RN_MAX_NV(T)) return YMK_E_BADARG;
     else {
-        if (p.nv > NV) return rn_launch<T, V, QUANT, NV * 2>(p, a, stream);
-        hipLaunchKernelGGL((rms_norm_kernel<T, V, NV, QUANT>), dim3(p.grid), dim3(p.threads), 0, (hipStream_t)stream, a);
+        if (p.nv > NV) return rn_launch<T, EVEN, QUANT, NV * 2>(p, a, stream);
+        hipLaunchKernelGGL((rms_norm_kernel<T, EVEN, NV, QUANT>), dim3(p.grid), dim3(p.threads), 0, (hipStream_t)stream, a);
         return ymk_launch_status();
     }
 }
-template <typename T, int V, int NV = 1>
+template <typename T, bool EVEN, int NV = 1>
 int rn_launch_backward(const RnPlan& p, const RnBwdArgs& a, void* stream) {
-    if constexpr (NV > (V == 1 ? 16 : 4 * (int)sizeof(T) / 2)) return YMK_E_BADARG;
+    if constexpr (NV > RN_MAX_NV_BWD(T)) return YMK_E_BADARG;
     else {
-        if (p.nv > NV) return rn_launch_backward<T, V, NV * 2>(p, a, stream);
-        const size_t lds = p.threads > p.group && a.part ? (size_t)p.threads * V * NV * sizeof(float) : 0;
-        hipLaunchKernelGGL((rms_norm_backward_kernel<T, V, NV>), dim3(p.grid), dim3(p.threads), lds, (hipStream_t)stream, a);
+        if (p.nv > NV) return rn_launch_backward<T, EVEN, NV * 2>(p, a, stream);
+        const size_t lds = p.threads > p.group && a.part ? (size_t)p.threads * (16 / sizeof(T)) * NV * sizeof(float) : 0;
+        hipLaunchKernelGGL((rms_norm_backward_kernel<T, EVEN, NV>), dim3(p.grid), dim3(p.threads), lds, (hipStream_t)stream, a);
         return ymk_launch_status();
     }
 }
-inline int rn_vec(int32_t dtype, int32_t C) { return C % (dtype == YMK_F32 ? 4 : 8) == 0 ? (dtype == YMK_F32 ? 4 : 8) : 1; }
-inline int rn_max_nv(int32_t dtype, int V) { return V == 1 ? 16 : dtype == YMK_F32 ? 8 : 4; }
 
 int rms_norm_any(bool quant, int32_t dtype, const void* x, int32_t ldx, const void* residual, int32_t ldr, void* h, int32_t ldh, void* y, int32_t ldy,
                  float* stat, int64_t rows, int32_t C, const float* weight, float eps, void* stream) {
@@ -338,18 +364,17 @@ int rms_norm_any(bool quant, int32_t dtype, const void* x, int32_t ldx, const vo
     if (rows == 0) return YMK_OK;
     if (!weight || rn_bad(x, ldx, C, es) || (residual && (rn_bad(residual, ldr, C, es) || rn_bad(h, ldh, C, es))) || rn_bad(y, ldy, C, quant ? 1 : es) || (quant && !stat))
         return YMK_E_BADARG;
-    int V = rn_vec(dtype, C);
-    if (ldx % V || !rn_al(x, 16) || (residual && (ldr % V || ldh % V || !rn_al(residual, 16) || !rn_al(h, 16))) || ldy % V || !rn_al(y, quant ? V : 16)) V = 1;
-    const RnArgs a{x, residual, h, y, stat, weight, rows, ldx, ldr, ldh, ldy, C, 0, eps};
-    RnPlan p = rn_plan(rows, (C + V - 1) / V, rn_max_nv(dtype, V), RN_MAX_WAVES, RN_MAX_GROUPS);
-    RnArgs b = a;
-    b.group = p.group;
+    const int V = 16 / es;
+    const bool even = C % V == 0 && ldx % V == 0 && rn_al(x, 16) && (!residual || (ldr % V == 0 && ldh % V == 0 && rn_al(residual, 16) && rn_al(h, 16))) &&
+                      ldy % V == 0 && rn_al(y, quant ? V : 16);
+    const RnPlan p = rn_plan(rows, (C + V - 1) / V, dtype == YMK_F32 ? RN_MAX_NV(float) : RN_MAX_NV(h16_t), RN_MAX_WAVES, RN_MAX_GROUPS);
+    const RnArgs a{x, residual, h, y, stat, weight, rows, ldx, ldr, ldh, ldy, C, p.group, eps};
     if (dtype == YMK_F32) {
-        if (quant) return V == 1 ? rn_launch<float, 1, true>(p, b, stream) : rn_launch<float, 4, true>(p, b, stream);
-        return V == 1 ? rn_launch<float, 1, false>(p, b, stream) : rn_launch<float, 4, false>(p, b, stream);
+        if (quant) return even ? rn_launch<float, true, true>(p, a, stream) : rn_launch<float, false, true>(p, a, stream);
+        return even ? rn_launch<float, true, false>(p, a, stream) : rn_launch<float, false, false>(p, a, stream);
     }
-    if (quant) return V == 1 ? rn_launch<h16_t, 1, true>(p, b, stream) : rn_launch<h16_t, 8, true>(p, b, stream);
-    return V == 1 ? rn_launch<h16_t, 1, false>(p, b, stream) : rn_launch<h16_t, 8, false>(p, b, stream);
+    if (quant) return even ? rn_launch<h16_t, true, true>(p, a, stream) : rn_launch<h16_t, false, true>(p, a, stream);
+    return even ? rn_launch<h16_t, true, false>(p, a, stream) : rn_launch<h16_t, false, false>(p, a, stream);
 }
 
 }  // namespace
@@ -377,17 +402,18 @@ extern "C" int ymk_rms_norm_backward(int32_t dtype, const void* dy, int32_t lddy
         return YMK_E_BADARG;
     if (dweight && rows > 0 && (!workspace || workspace_bytes < ymk_rms_norm_backward_workspace_bytes(rows, C))) return YMK_E_WORKSPACE;
     if (rows > 0) {
-        int V = rn_vec(dtype, C);
-        if (lddy % V || ldh % V || lddx % V || !rn_al(dy, 16) || !rn_al(h, 16) || !rn_al(dx, 16) || (dres && (lddr % V || !rn_al(dres, 16)))) V = 1;
-        const RnPlan p = rn_plan(rows, (C + V - 1) / V, rn_max_nv(dtype, V), (int64_t)RN_BWD_BLOCKS * 4, RN_BWD_BLOCKS);
+        const int V = 16 / es;
+        const bool even = C % V == 0 && lddy % V == 0 && ldh % V == 0 && lddx % V == 0 && rn_al(dy, 16) && rn_al(h, 16) && rn_al(dx, 16) &&
+                          (!dres || (lddr % V == 0 && rn_al(dres, 16)));
+        const RnPlan p = rn_plan(rows, (C + V - 1) / V, dtype == YMK_F32 ? RN_MAX_NV_BWD(float) : RN_MAX_NV_BWD(h16_t), (int64_t)RN_BWD_BLOCKS * 4, RN_BWD_BLOCKS);
         const RnBwdArgs a{dy, h, rstd, weight, dres, dx, dweight ? static_cast<float*>(workspace) : nullptr, rows, lddy, ldh, lddr, lddx, C, p.group};
-        const int rc = dtype == YMK_F32 ? (V == 1 ? rn_launch_backward<float, 1>(p, a, stream) : rn_launch_backward<float, 4>(p, a, stream))
-                                        : (V == 1 ? rn_launch_backward<h16_t, 1>(p, a, stream) : rn_launch_backward<h16_t, 8>(p, a, stream));
+        const int rc = dtype == YMK_F32 ? (even ? rn_launch_backward<float, true>(p, a, stream) : rn_launch_backward<float, false>(p, a, stream))
+                                        : (even ? rn_launch_backward<h16_t, true>(p, a, stream) : rn_launch_backward<h16_t, false>(p, a, stream));
         if (rc != YMK_OK || !dweight) return rc;
-        hipLaunchKernelGGL(rms_norm_dweight_kernel, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, (hipStream_t)stream, static_cast<const float*>(workspace), (int)p.grid,
+        hipLaunchKernelGGL(rms_norm_dweight_kernel, dim3((unsigned)((C + 15) / 16)), dim3(1024), 0, (hipStream_t)stream, static_cast<const float*>(workspace), (int)p.grid,
                            (int)C, dweight);
     } else if (dweight) {   // no rows: the sum over none of them
-        hipLaunchKernelGGL(rms_norm_dweight_kernel, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, (hipStream_t)stream, static_cast<const float*>(nullptr), 0, (int)C, dweight);
+        hipLaunchKernelGGL(rms_norm_dweight_kernel, dim3((unsigned)((C + 15) / 16)), dim3(1024), 0, (hipStream_t)stream, static_cast<const float*>(nullptr), 0, (int)C, dweight);
     }
     return ymk_launch_status();
 }

@@ -2,6 +2,7 @@
 // the weighted sum back, with their gradients.  Nothing here multiplies matrices: the sort is bound by latency (a launch, two dependent reads),
 // the moves by memory — each row is read once and written once.
 #include "ymk_common.h"
+#include "rows.h"
 #include "../../include/ymk_tokens.h"
 
 #ifndef YMK_MAX_BLOCKS
@@ -124,39 +125,48 @@ __global__ __launch_bounds__(1024) void token_sort_one_kernel(SortArgs a) {
     sort_place<16>(a, 0, a.pairs, count, start);
 }
 
-__global__ __launch_bounds__(256) void token_sort_count_kernel(SortArgs a) {
-    __shared__ int32_t count[4][YMK_TOKEN_MAX_E + 1];
+__global__ __launch_bounds__(1024) void token_sort_count_kernel(SortArgs a) {
+    __shared__ int32_t count[16][YMK_TOKEN_MAX_E + 1];
     const int64_t p0 = (int64_t)blockIdx.x * a.per, p1 = min(a.pairs, p0 + a.per);
-    sort_count<4>(a, p0, p1, count);
-    for (int e = threadIdx.x; e <= a.E; e += 256) a.hist[(size_t)blockIdx.x * (a.E + 1) + e] = count[0][e] + count[1][e] + count[2][e] + count[3][e];
+    sort_count<16>(a, p0, p1, count);
+    for (int e = threadIdx.x; e <= a.E; e += 1024) {
+        int n = 0;
+        for (int i = 0; i < 16; ++i) n += count[i][e];
+        a.hist[(size_t)blockIdx.x * (a.E + 1) + e] = n;
+    }
 }
 
-__global__ __launch_bounds__(256) void token_sort_place_kernel(SortArgs a) {
-    __shared__ int32_t count[4][YMK_TOKEN_MAX_E + 1];
+__global__ __launch_bounds__(1024) void token_sort_place_kernel(SortArgs a) {
+    __shared__ int32_t count[16][YMK_TOKEN_MAX_E + 1];
     __shared__ int32_t total[YMK_TOKEN_MAX_E + 1], mine[YMK_TOKEN_MAX_E + 1], start[YMK_TOKEN_MAX_E + 1];
-    for (int e = threadIdx.x; e <= a.E; e += 256) total[e] = mine[e] = 0;
+    for (int e = threadIdx.x; e <= a.E; e += 1024) total[e] = mine[e] = 0;
     __syncthreads();
-    // strands of workgroups per key: 256 / (keys rounded up to a power of two), added up in LDS (integers)
+    // strands of workgroups per key: 1024 / (keys rounded up to a power of two), four histograms of a strand in flight, added up in LDS (integers)
     int keys = 1;
-    while (keys <= a.E && keys < 256) keys <<= 1;
-    const int strands = 256 / keys, s = threadIdx.x / keys;
-    for (int e = threadIdx.x & (keys - 1); e <= a.E; e += keys) {
+    while (keys <= a.E && keys < 512) keys <<= 1;
+    const int strands = 1024 / keys, s = threadIdx.x / keys, e = threadIdx.x & (keys - 1), n = gridDim.x;
+    if (e <= a.E) {
         int all = 0, before = 0;
-        for (int b = s; b < (int)gridDim.x; b += strands) {
-            const int n = a.hist[(size_t)b * (a.E + 1) + e];
-            all += n;
-            before += b < (int)blockIdx.x ? n : 0;
+        for (int b = s; b < n; b += 4 * strands) {
+            int h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = b + i * strands < n ? a.hist[(size_t)(b + i * strands) * (a.E + 1) + e] : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                all += h[i];
+                before += b + i * strands < (int)blockIdx.x ? h[i] : 0;
+            }
         }
         atomicAdd(&total[e], all);
         atomicAdd(&mine[e], before);
     }
     __syncthreads();
     sort_starts(total, a.E, start, blockIdx.x == 0 ? a.offsets : nullptr);
-    for (int e = threadIdx.x; e <= a.E; e += 256) start[e] += mine[e];
+    for (int i = threadIdx.x; i <= a.E; i += 1024) start[i] += mine[i];
     __syncthreads();
     const int64_t p0 = (int64_t)blockIdx.x * a.per, p1 = min(a.pairs, p0 + a.per);
-    sort_count<4>(a, p0, p1, count);
-    sort_place<4>(a, p0, p1, count, start);
+    sort_count<16>(a, p0, p1, count);
+    sort_place<16>(a, p0, p1, count, start);
 }
 
 // -------------------------------------------------------------------------------------------------------- dispatch
@@ -165,23 +175,25 @@ struct MoveArgs {
     char* xs;
     const float* scale;
     float* xs_scale;
-    const int32_t* row;
+    const int32_t* rows;
     int64_t ldx, ldxs, tokens;   // strides in bytes
-    int32_t units, top_k;        // units of sizeof(U) bytes a row
+    int32_t units, row, top_k;   // units of sizeof(U) bytes that cover a row of so many bytes
 };
 
-// One unit of a token per lane: read once, written to the rows of the token's choices.
+// One unit of a token per lane: read once, written to the rows of the token's choices.  A unit may start at any byte; the last one of a row ends with
+// it, over bytes that the one before it writes as well (the same ones).
 template <typename U>
 __global__ __launch_bounds__(256) void token_dispatch_kernel(MoveArgs a) {
+    typedef U Any __attribute__((aligned(1)));
     const int64_t n = a.tokens * a.units;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t t = n < 0x7fffffff ? (uint32_t)i / (uint32_t)a.units : i / a.units;
-        const int j = (int)(i - t * a.units);
-        const U v = *reinterpret_cast<const U*>(a.x + t * a.ldx + (int64_t)j * sizeof(U));
+        const int j = (int)(i - t * a.units), at = min(j * (int)sizeof(U), a.row - (int)sizeof(U));
+        const U v = *reinterpret_cast<const Any*>(a.x + t * a.ldx + at);
         for (int k = 0; k < a.top_k; ++k) {
-            const int64_t r = a.row[t * a.top_k + k];
+            const int64_t r = a.rows[t * a.top_k + k];
             if (r < 0) continue;
-            *reinterpret_cast<U*>(a.xs + r * a.ldxs + (int64_t)j * sizeof(U)) = v;
+            *reinterpret_cast<Any*>(a.xs + r * a.ldxs + at) = v;
             if (a.scale && j == 0) a.xs_scale[r] = a.scale[t];
         }
     }
@@ -194,40 +206,48 @@ struct CombineArgs {
     const float* w;
     void* y;
     int64_t tokens;
-    int32_t ldys, ldy, units, top_k;
+    int32_t ldys, ldy, units, C, top_k;
 };
 
+// V channels at p (any alignment): 16 bytes, or one
 template <typename T, int V>
 __device__ __forceinline__ void tk_load(const T* p, float (&v)[V]) {
     if constexpr (V == 1) v[0] = to_f32(*p);
-    else load_vec_f32(p, v);
+    else row_load<T, false>(p, V, v);
 }
 template <typename T, int V>
 __device__ __forceinline__ void tk_store(T* p, const float (&v)[V]) {
     if constexpr (V == 1) from_f32(*p, v[0]);
-    else store_vec_f32(p, v);
+    else row_store<T, false>(p, V, v);
 }
 
-// V channels of a token per lane, the choices added in their order in fp32
-template <typename T, int V>
+// V channels of a token per lane (the last ones of a row end with it, over channels that the lane before has as well), KU choices in flight at a time,
+// added in their order in fp32.  A pair without a row reads row 0 (there is one: the token's own pairs count) and takes nothing of it.
+template <typename T, int V, int KU>
 __global__ __launch_bounds__(256) void token_combine_kernel(CombineArgs a) {
     const int64_t n = a.tokens * a.units;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t t = n < 0x7fffffff ? (uint32_t)i / (uint32_t)a.units : i / a.units;
-        const int j = (int)(i - t * a.units);
+        const int c = min((int)(i - t * a.units) * V, a.C - V);
         float s[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) s[e] = 0.f;
-        for (int k = 0; k < a.top_k; ++k) {
-            const int64_t r = a.row[t * a.top_k + k];
-            if (r < 0) continue;
-            const float w = a.w ? a.w[t * a.top_k + k] : 1.0f;
-            float v[V];
-            tk_load<T, V>(static_cast<const T*>(a.ys) + r * a.ldys + (int64_t)j * V, v);
+        for (int k0 = 0; k0 < a.top_k; k0 += KU) {
+            float v[KU][V], w[KU];
+            int64_t r[KU];
 #pragma unroll
-            for (int e = 0; e < V; ++e) s[e] = fmaf(w, v[e], s[e]);
+            for (int k = 0; k < KU; ++k) {
+                r[k] = k0 + k < a.top_k ? a.row[t * a.top_k + k0 + k] : -1;
+                w[k] = a.w && k0 + k < a.top_k ? a.w[t * a.top_k + k0 + k] : 1.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < KU; ++k) tk_load<T, V>(static_cast<const T*>(a.ys) + (r[k] < 0 ? 0 : r[k]) * a.ldys + c, v[k]);
+#pragma unroll
+            for (int k = 0; k < KU; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[e] = r[k] < 0 ? s[e] : fmaf(w[k], v[k][e], s[e]);
         }
-        tk_store<T, V>(static_cast<T*>(a.y) + t * a.ldy + (int64_t)j * V, s);
+        tk_store<T, V>(static_cast<T*>(a.y) + t * a.ldy + c, s);
     }
 }
 
@@ -239,11 +259,11 @@ struct CombineBwdArgs {
     void* dys;
     float* dw;
     int64_t tokens;
-    int32_t lddy, ldys, lddys, units, top_k, group;
+    int32_t lddy, ldys, lddys, units, C, top_k, group;
 };
 
 // A token belongs to `group` lanes (8..64) of a wave: per choice they scale the token's dy into its row and add up <dy, ys>.  dy of a token stays
-// in the cache over its choices.
+// in the cache over its choices.  Where the last unit of a row overlaps the one before it, the shared channels count once.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void token_combine_backward_kernel(CombineBwdArgs a) {
     const int lane = threadIdx.x & (a.group - 1), per = 256 / a.group;
@@ -254,15 +274,16 @@ __global__ __launch_bounds__(256) void token_combine_backward_kernel(CombineBwdA
             if (r >= 0) {
                 const float w = a.w[t * a.top_k + k];
                 for (int j = lane; j < a.units; j += a.group) {
+                    const int c = min(j * V, a.C - V), again = j * V - c;
                     float d[V], v[V];
-                    tk_load<T, V>(static_cast<const T*>(a.dy) + t * a.lddy + (int64_t)j * V, d);
-                    tk_load<T, V>(static_cast<const T*>(a.ys) + r * a.ldys + (int64_t)j * V, v);
+                    tk_load<T, V>(static_cast<const T*>(a.dy) + t * a.lddy + c, d);
+                    tk_load<T, V>(static_cast<const T*>(a.ys) + r * a.ldys + c, v);
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        dot = fmaf(d[e], v[e], dot);
+                        dot = e < again ? dot : fmaf(d[e], v[e], dot);
                         d[e] *= w;
                     }
-                    tk_store<T, V>(static_cast<T*>(a.dys) + r * a.lddys + (int64_t)j * V, d);
+                    tk_store<T, V>(static_cast<T*>(a.dys) + r * a.lddys + c, d);
                 }
             }
             for (int o = a.group >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
@@ -276,6 +297,15 @@ inline bool tk_bad_plan(int64_t tokens, int32_t top_k) { return tokens < 0 || to
 inline unsigned tk_blocks(int64_t lanes) {
     const int64_t n = (lanes + 255) / 256;
     return (unsigned)(n < TK_MAX_BLOCKS ? n : TK_MAX_BLOCKS);
+}
+
+template <typename T, int V>
+int tk_combine(const CombineArgs& a, void* stream) {
+    const dim3 grid(tk_blocks(a.tokens * a.units)), block(256);
+    if (a.top_k == 1) hipLaunchKernelGGL((token_combine_kernel<T, V, 1>), grid, block, 0, (hipStream_t)stream, a);
+    else if (a.top_k == 2) hipLaunchKernelGGL((token_combine_kernel<T, V, 2>), grid, block, 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((token_combine_kernel<T, V, 4>), grid, block, 0, (hipStream_t)stream, a);
+    return ymk_launch_status();
 }
 
 }  // namespace
@@ -296,12 +326,12 @@ extern "C" int ymk_token_sort(const void* idx, int32_t idx_bytes, int64_t tokens
         return ymk_launch_status();
     }
     if (!workspace || workspace_bytes < ymk_token_sort_workspace_bytes(tokens, top_k, E)) return YMK_E_WORKSPACE;
-    int64_t blocks = (pairs + 1023) / 1024;
+    int64_t blocks = (pairs + 2047) / 2048;
     if (blocks > TK_SORT_BLOCKS) blocks = TK_SORT_BLOCKS;
     a.per = (int32_t)((pairs + blocks - 1) / blocks);
     blocks = (pairs + a.per - 1) / a.per;
-    hipLaunchKernelGGL(token_sort_count_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
-    hipLaunchKernelGGL(token_sort_place_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(token_sort_count_kernel, dim3((unsigned)blocks), dim3(1024), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(token_sort_place_kernel, dim3((unsigned)blocks), dim3(1024), 0, (hipStream_t)stream, a);
     return ymk_launch_status();
 }
 
@@ -311,9 +341,9 @@ extern "C" int ymk_token_dispatch(const void* x, int64_t ldx_bytes, int64_t row_
         return YMK_E_BADARG;
     if (tokens == 0) return YMK_OK;
     if (!x || !xs || !row) return YMK_E_BADARG;
-    int u = 16;   // widest unit that divides the row, both strides and both addresses
-    while (row_bytes % u || ldx_bytes % u || ldxs_bytes % u || !tk_al(x, u) || !tk_al(xs, u)) u >>= 1;
-    const MoveArgs a{static_cast<const char*>(x), static_cast<char*>(xs), scale, xs_scale, row, ldx_bytes, ldxs_bytes, tokens, (int32_t)(row_bytes / u), top_k};
+    int u = 16;   // widest unit that a row holds
+    while (u > row_bytes) u >>= 1;
+    const MoveArgs a{static_cast<const char*>(x), static_cast<char*>(xs), scale, xs_scale, row, ldx_bytes, ldxs_bytes, tokens, (int32_t)((row_bytes + u - 1) / u), (int32_t)row_bytes, top_k};
     const dim3 grid(tk_blocks(tokens * a.units)), block(256);
     if (u == 16) hipLaunchKernelGGL(token_dispatch_kernel<u32x4>, grid, block, 0, (hipStream_t)stream, a);
     else if (u == 8) hipLaunchKernelGGL(token_dispatch_kernel<u32x2>, grid, block, 0, (hipStream_t)stream, a);
@@ -329,16 +359,10 @@ extern "C" int ymk_token_combine(int32_t dtype, const void* ys, int32_t ldys, co
     if (tokens == 0) return YMK_OK;
     const int es = dtype == YMK_F32 ? 4 : 2;
     if (!ys || !row || !y || !tk_al(ys, es) || !tk_al(y, es)) return YMK_E_BADARG;
-    int V = 16 / es;
-    if (C % V || ldys % V || ldy % V || !tk_al(ys, 16) || !tk_al(y, 16)) V = 1;
-    const CombineArgs a{ys, row, w, y, tokens, ldys, ldy, C / V, top_k};
-    const dim3 grid(tk_blocks(tokens * a.units)), block(256);
-    if (dtype == YMK_F32) {
-        if (V == 1) hipLaunchKernelGGL((token_combine_kernel<float, 1>), grid, block, 0, (hipStream_t)stream, a);
-        else hipLaunchKernelGGL((token_combine_kernel<float, 4>), grid, block, 0, (hipStream_t)stream, a);
-    } else if (V == 1) hipLaunchKernelGGL((token_combine_kernel<h16_t, 1>), grid, block, 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((token_combine_kernel<h16_t, 8>), grid, block, 0, (hipStream_t)stream, a);
-    return ymk_launch_status();
+    const int V = C >= 16 / es ? 16 / es : 1;
+    const CombineArgs a{ys, row, w, y, tokens, ldys, ldy, (C + V - 1) / V, C, top_k};
+    if (dtype == YMK_F32) return V == 1 ? tk_combine<float, 1>(a, stream) : tk_combine<float, 4>(a, stream);
+    return V == 1 ? tk_combine<h16_t, 1>(a, stream) : tk_combine<h16_t, 8>(a, stream);
 }
 
 extern "C" int ymk_token_combine_backward(int32_t dtype, const void* dy, int32_t lddy, const void* ys, int32_t ldys, const int32_t* row, const float* w,
@@ -347,9 +371,8 @@ extern "C" int ymk_token_combine_backward(int32_t dtype, const void* dy, int32_t
     if (tokens == 0) return YMK_OK;
     const int es = dtype == YMK_F32 ? 4 : 2;
     if (!dy || !ys || !row || !w || !dys || !dw || !tk_al(dy, es) || !tk_al(ys, es) || !tk_al(dys, es)) return YMK_E_BADARG;
-    int V = 16 / es;
-    if (C % V || lddy % V || ldys % V || lddys % V || !tk_al(dy, 16) || !tk_al(ys, 16) || !tk_al(dys, 16)) V = 1;
-    CombineBwdArgs a{dy, ys, row, w, dys, dw, tokens, lddy, ldys, lddys, C / V, top_k, 8};
+    const int V = C >= 16 / es ? 16 / es : 1;
+    CombineBwdArgs a{dy, ys, row, w, dys, dw, tokens, lddy, ldys, lddys, (C + V - 1) / V, C, top_k, 8};
     while (a.group < 64 && a.group < a.units) a.group *= 2;
     const dim3 grid(tk_blocks(tokens * a.group)), block(256);
     if (dtype == YMK_F32) {

@@ -34,6 +34,7 @@ C-side, read by libymk itself at first use (A/B switches of one kernel's launch 
     YMK_ATTN_WAVES          0         5 | 6 forces five- / six-wave workgroups in the resident area attention      csrc/attn.hip
     YMK_WS_MIN_TILES, YMK_GLDS_MIN_TILES, YMK_GLDS_MIN_K, YMK_GLDS_BIG_MIN_TILES, YMK_GLDS_SMALL_BELOW, YMK_GLDS_TILE, YMK_GLDS_TAP_OUTER,
     YMK_GLDS_THREE_STAGE    —         kernel-selection thresholds of the convolution cores                         csrc/conv.hip, conv_glds.hip
+    YMK_EXPERT_TILE         0         16 | 64 | 128 | 256: that tile for every size of the experts' product            csrc/expert.hip
     YMK_DW_WG_TARGET        0         tiles per workgroup of the depthwise stencil                                 csrc/dwconv.hip
 """
 from __future__ import annotations
