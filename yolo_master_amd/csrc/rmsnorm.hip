@@ -20,7 +20,7 @@
 
 #define RN_MAX_NV(T) (2 * (int)sizeof(T))    // vectors a lane holds at most: 32 values,
 #define RN_MAX_NV_BWD(T) ((int)sizeof(T))    // 16 in the gradient, which keeps five of each (128 registers)
-#define RN_TINY 0x1.cp-118f   // 448 * 2^-126: below it the scale would be subnormal and its reciprocal infinite
+#define RN_SMALL 0x1.cp-118f   // 448 * 2^-126: below it the scale would be subnormal and its reciprocal infinite
 
 namespace {
 
@@ -30,28 +30,36 @@ __device__ __forceinline__ float rn_round(float v) {
     if constexpr (sizeof(T) == 4) return v;
     else return h16_to_f32(f32_to_h16(v));
 }
-// the first n of V values in e4m3
+// V values in e4m3 (TINY: the first n)
 __device__ __forceinline__ uint32_t rn_e4m3(float a, float b, float c, float d) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
-template <bool EVEN, int V>
+template <bool TINY, int V>
 __device__ __forceinline__ void rn_store_e4m3(uint8_t* p, int n, const float (&v)[V]) {
-    if (EVEN || n >= V) {
-        if constexpr (V == 8) {
-            const u32x2 w{rn_e4m3(v[0], v[1], v[2], v[3]), rn_e4m3(v[4], v[5], v[6], v[7])};
-            if constexpr (EVEN) *reinterpret_cast<u32x2*>(p) = w;
-            else *reinterpret_cast<u32x2_u*>(p) = w;
-        } else {
-            const uint32_t w = rn_e4m3(v[0], v[1], v[2], v[3]);
-            if constexpr (EVEN) *reinterpret_cast<uint32_t*>(p) = w;
-            else *reinterpret_cast<u32_u*>(p) = w;
-        }
+    if constexpr (!TINY) {
+        if constexpr (V == 8) *reinterpret_cast<u32x2_u*>(p) = u32x2{rn_e4m3(v[0], v[1], v[2], v[3]), rn_e4m3(v[4], v[5], v[6], v[7])};
+        else *reinterpret_cast<u32_u*>(p) = rn_e4m3(v[0], v[1], v[2], v[3]);
     } else {
 #pragma unroll
-        for (int e = 0; e < V - 1; ++e)
+        for (int e = 0; e < V; ++e)
             if (e < n) p[e] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[e], 0.f, 0, false);
     }
 }
+
+// A lane's vectors of a row: vector i covers columns [at(i), at(i) + V), of which the first again(i) belong to an earlier vector (all V: the lane has none).
+// EVEN widths have whole vectors only; TINY ones less than one.
+enum { RN_EVEN, RN_RAGGED, RN_TINY };
+template <int W, int V>
+struct RnCols {
+    int first, step, C;   // column of vector 0, and from one vector to the next
+    __device__ __forceinline__ int at(int i) const { return W == RN_TINY ? 0 : min(first + i * step, C - V); }
+    __device__ __forceinline__ bool mine(int i) const { return first + i * step < C; }
+    __device__ __forceinline__ bool counts(int i, int e) const {   // element e of vector i is in the row and no other lane's
+        if (W == RN_EVEN) return mine(i);
+        if (W == RN_TINY) return mine(i) && e < C;
+        return e >= first + i * step - at(i);
+    }
+};
 
 // Sum (and, below, largest bit pattern) over the group of a lane: lanes [l - l % group, + group) of a wave, or all `group` lanes of the workgroup
 // through LDS (two slots used in turn: one barrier a reduction).  Every lane gets the result of the same tree: bit-identical within the group.
@@ -89,59 +97,50 @@ struct RnArgs {
     float eps;
 };
 
-template <typename T, bool EVEN, int NV, bool QUANT>
-__global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
+template <typename T, int W, int NV, bool QUANT>
+__global__ __launch_bounds__(NV == RN_MAX_NV(T) ? 256 : 1024) void rms_norm_kernel(RnArgs a) {
     constexpr int V = 16 / sizeof(T);
+    constexpr bool TINY = W == RN_TINY;
     __shared__ float part[2][16];
     RnGroup g{a.group, 0, part};
     const int lane = threadIdx.x & (a.group - 1), per = blockDim.x / a.group;
+    const RnCols<W, V> cols{lane * V, a.group * V, a.C};
     const T* x = static_cast<const T*>(a.x);
     const T* res = static_cast<const T*>(a.res);
     float w[NV][V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (lane + i * a.group) * V;
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) w[i][e] = c + e < a.C ? a.weight[c + e] : 0.f;
-    }
+        for (int e = 0; e < V; ++e) w[i][e] = a.weight[TINY ? min(e, a.C - 1) : cols.at(i) + e];
     const float inv_c = 1.0f / (float)a.C;
     for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < a.rows; r0 += (int64_t)gridDim.x * per) {   // the same trips for the whole workgroup
-        const int64_t r = r0 + threadIdx.x / a.group;
-        const int cols = r < a.rows ? a.C : 0;
-        float v[NV][V];
-        float ss = 0.f;
+        const int64_t r = min(r0 + threadIdx.x / a.group, a.rows - 1);                            // a group behind the last row repeats it
+        const bool live = r0 + threadIdx.x / a.group < a.rows;
+        u32x4 raw[NV], add[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * a.group) * V;
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[i][e] = 0.f;
-            if (c < cols) row_load<T, EVEN>(x + r * a.ldx + c, cols - c, v[i]);
-        }
+        for (int i = 0; i < NV; ++i) raw[i] = row_load<T, TINY>(x + r * a.ldx + cols.at(i), a.C);
         if (res) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (lane + i * a.group) * V;
-                if (c < cols) {
-                    float b[V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) b[e] = 0.f;
-                    row_load<T, EVEN>(res + r * a.ldr + c, cols - c, b);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) v[i][e] = rn_round<T>(v[i][e] + b[e]);
-                }
-            }
+            for (int i = 0; i < NV; ++i) add[i] = row_load<T, TINY>(res + r * a.ldr + cols.at(i), a.C);
         }
+        float v[NV][V], ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            row_widen(raw[i], v[i]);
+            if (res) {
+                float b[V];
+                row_widen(add[i], b);
 #pragma unroll
-            for (int e = 0; e < V; ++e) ss = fmaf(v[i][e], v[i][e], ss);
+                for (int e = 0; e < V; ++e) v[i][e] = rn_round<T>(v[i][e] + b[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) ss = cols.counts(i, e) ? fmaf(v[i][e], v[i][e], ss) : ss;
+        }
         const float rstd = 1.0f / sqrtf(g.sum(ss) * inv_c + a.eps);
         if (res) {   // after the reduction: every lane of the group has read what h may alias
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (lane + i * a.group) * V;
-                if (c < cols) row_store<T, EVEN>(static_cast<T*>(a.h) + r * a.ldh + c, cols - c, v[i]);
-            }
+            for (int i = 0; i < NV; ++i)
+                if (live && cols.mine(i)) row_store<T, TINY>(static_cast<T*>(a.h) + r * a.ldh + cols.at(i), a.C, v[i]);
         }
         float top = 0.f;
 #pragma unroll
@@ -149,7 +148,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 v[i][e] = v[i][e] * rstd * w[i][e];
-                if constexpr (QUANT) {
+                if constexpr (QUANT) {   // an element that two lanes hold does no harm; TINY zeros neither, unless the row's scale is not finite
                     const float m = __uint_as_float(__float_as_uint(v[i][e]) & 0x7fffffffu);
                     top = __float_as_uint(m) > __float_as_uint(top) ? m : top;
                 }
@@ -157,25 +156,22 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(RnArgs a) {
         float stat = rstd;
         if constexpr (QUANT) {
             top = g.top(top);
-            const float scale = top < RN_TINY ? 1.0f : top * (1.0f / 448.0f) < __uint_as_float(0x7f800000u) ? top / 448.0f : __uint_as_float(0x7fc00000u);
+            const float scale = top < RN_SMALL ? 1.0f : top * (1.0f / 448.0f) < __uint_as_float(0x7f800000u) ? top / 448.0f : __uint_as_float(0x7fc00000u);
             stat = scale;
             // y * (1 / scale) is within 2^-23 of y / scale and never above 448 * (1 + 2^-22), which rounds to 448: no clamp, and NaN stays NaN
             const float inv = 1.0f / scale;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (lane + i * a.group) * V;
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[i][e] = top < RN_TINY ? 0.f : v[i][e] * inv;
-                if (c < cols) rn_store_e4m3<EVEN>(static_cast<uint8_t*>(a.y) + r * a.ldy + c, cols - c, v[i]);
+                for (int e = 0; e < V; ++e) v[i][e] = top < RN_SMALL ? 0.f : v[i][e] * inv;
+                if (live && cols.mine(i)) rn_store_e4m3<TINY>(static_cast<uint8_t*>(a.y) + r * a.ldy + cols.at(i), a.C, v[i]);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (lane + i * a.group) * V;
-                if (c < cols) row_store<T, EVEN>(static_cast<T*>(a.y) + r * a.ldy + c, cols - c, v[i]);
-            }
+            for (int i = 0; i < NV; ++i)
+                if (live && cols.mine(i)) row_store<T, TINY>(static_cast<T*>(a.y) + r * a.ldy + cols.at(i), a.C, v[i]);
         }
-        if (a.stat && lane == 0 && cols) a.stat[r] = stat;
+        if (a.stat && lane == 0 && live) a.stat[r] = stat;
     }
 }
 
@@ -193,84 +189,84 @@ struct RnBwdArgs {
 
 // dx of a row in one pass over it; dweight: a lane sums its columns over the rows it walks, the groups of a workgroup are added in a fixed
 // order through LDS, and each workgroup leaves one partial row that rms_norm_dweight_kernel adds up — no atomics, the same bits every time.
-template <typename T, bool EVEN, int NV>
+template <typename T, int W, int NV>
 __global__ __launch_bounds__(1024) void rms_norm_backward_kernel(RnBwdArgs a) {
     constexpr int V = 16 / sizeof(T);
+    constexpr bool TINY = W == RN_TINY;
     __shared__ float part[2][16];
     extern __shared__ float dw_lds[];   // [groups of the workgroup][columns of a group]
     RnGroup g{a.group, 0, part};
     const int lane = threadIdx.x & (a.group - 1), per = blockDim.x / a.group;
+    const RnCols<W, V> cols{lane * V, a.group * V, a.C};
     const T* dyp = static_cast<const T*>(a.dy);
     const T* hp = static_cast<const T*>(a.h);
     const T* drp = static_cast<const T*>(a.dres);
     float w[NV][V], dw[NV][V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (lane + i * a.group) * V;
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            w[i][e] = c + e < a.C ? a.weight[c + e] : 0.f;
+            w[i][e] = a.weight[TINY ? min(e, a.C - 1) : cols.at(i) + e];
             dw[i][e] = 0.f;
         }
-    }
     const float inv_c = 1.0f / (float)a.C;
     for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < a.rows; r0 += (int64_t)gridDim.x * per) {   // the same trips for the whole workgroup
-        const int64_t r = r0 + threadIdx.x / a.group;
-        const int cols = r < a.rows ? a.C : 0;
-        float n[NV][V], d[NV][V], o[NV][V];
-        const float rstd = cols ? a.rstd[r] : 0.f;
+        const int64_t r = min(r0 + threadIdx.x / a.group, a.rows - 1);                            // a group behind the last row repeats it
+        const bool live = r0 + threadIdx.x / a.group < a.rows;
+        u32x4 hr[NV], dr[NV], orr[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * a.group) * V;
-#pragma unroll
-            for (int e = 0; e < V; ++e) n[i][e] = d[i][e] = o[i][e] = 0.f;
-            if (c < cols) {
-                row_load<T, EVEN>(hp + r * a.ldh + c, cols - c, n[i]);
-                row_load<T, EVEN>(dyp + r * a.lddy + c, cols - c, d[i]);
-                if (drp) row_load<T, EVEN>(drp + r * a.lddr + c, cols - c, o[i]);
-            }
+            hr[i] = row_load<T, TINY>(hp + r * a.ldh + cols.at(i), a.C);
+            dr[i] = row_load<T, TINY>(dyp + r * a.lddy + cols.at(i), a.C);
         }
-        float gn = 0.f;
+        if (drp) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i) orr[i] = row_load<T, TINY>(drp + r * a.lddr + cols.at(i), a.C);
+        }
+        const float rstd = a.rstd[r];
+        float n[NV][V], d[NV][V], gn = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            row_widen(hr[i], n[i]);
+            row_widen(dr[i], d[i]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 n[i][e] *= rstd;
-                dw[i][e] = fmaf(d[i][e], n[i][e], dw[i][e]);
+                dw[i][e] = live ? fmaf(d[i][e], n[i][e], dw[i][e]) : dw[i][e];
                 d[i][e] *= w[i][e];
-                gn = fmaf(d[i][e], n[i][e], gn);
+                gn = cols.counts(i, e) ? fmaf(d[i][e], n[i][e], gn) : gn;
             }
+        }
         gn = g.sum(gn) * inv_c;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * a.group) * V;
+            float o[V];
+            if (drp) row_widen(orr[i], o);
 #pragma unroll
-            for (int e = 0; e < V; ++e) o[i][e] = fmaf(rstd, fmaf(-n[i][e], gn, d[i][e]), o[i][e]);
-            if (c < cols) row_store<T, EVEN>(static_cast<T*>(a.dx) + r * a.lddx + c, cols - c, o[i]);
+            for (int e = 0; e < V; ++e) o[e] = fmaf(rstd, fmaf(-n[i][e], gn, d[i][e]), drp ? o[e] : 0.f);
+            if (live && cols.mine(i)) row_store<T, TINY>(static_cast<T*>(a.dx) + r * a.lddx + cols.at(i), a.C, o);
         }
     }
     if (!a.part) return;
     float* out = a.part + (size_t)blockIdx.x * a.C;
     if (per == 1) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * a.group) * V;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < V; ++e)
-                if (c + e < a.C) out[c + e] = dw[i][e];
-        }
+                if (cols.counts(i, e)) out[cols.at(i) + e] = dw[i][e];
         return;
     }
-    const int width = a.group * V * NV;   // columns a group holds, C or more
-    float* mine = dw_lds + (threadIdx.x / a.group) * width;
+    float* mine = dw_lds + (threadIdx.x / a.group) * a.C;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) mine[(lane + i * a.group) * V + e] = dw[i][e];
+        for (int e = 0; e < V; ++e)
+            if (cols.counts(i, e)) mine[cols.at(i) + e] = dw[i][e];
     __syncthreads();
     for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
         float s = 0.f;
-        for (int q = 0; q < per; ++q) s += dw_lds[q * width + c];
+        for (int q = 0; q < per; ++q) s += dw_lds[q * a.C + c];
         out[c] = s;
     }
 }
@@ -311,12 +307,13 @@ struct RnPlan {
     int group, nv, threads;
     unsigned grid;
 };
-inline RnPlan rn_plan(int64_t rows, int32_t vecs, int max_nv, int64_t max_waves, int64_t max_groups) {
+// max_nv / wide_nv: vectors a lane may hold in workgroups of up to 256 lanes and in wider ones.
+inline RnPlan rn_plan(int64_t rows, int32_t vecs, int max_nv, int wide_nv, int64_t max_waves, int64_t max_groups) {
     RnPlan p;
     const bool few = rows <= 512;
     p.group = 8;
     while (p.group < 64 && p.group * (few ? 1 : 2) < vecs) p.group *= 2;
-    while (p.group < 1024 && p.group * (few ? 1 : max_nv) < vecs) p.group *= 2;
+    while (p.group < 1024 && p.group * (few ? 1 : p.group < 256 ? max_nv : wide_nv) < vecs) p.group *= 2;
     p.nv = 1;
     while (p.group * p.nv < vecs) p.nv *= 2;
     p.threads = p.group > 64 ? p.group : 256;   // a group wider than a wave is a workgroup of its own
@@ -337,24 +334,35 @@ inline RnPlan rn_plan(int64_t rows, int32_t vecs, int max_nv, int64_t max_waves,
     return p;
 }
 
-template <typename T, bool EVEN, bool QUANT, int NV = 1>
+template <typename T, int W, bool QUANT, int NV = 1>
 int rn_launch(const RnPlan& p, const RnArgs& a, void* stream) {
-    if constexpr (NV > RN_MAX_NV(T)) return YMK_E_BADARG;
+    if constexpr (NV > (W == RN_TINY ? 1 : RN_MAX_NV(T))) return YMK_E_BADARG;
     else {
-        if (p.nv > NV) return rn_launch<T, EVEN, QUANT, NV * 2>(p, a, stream);
-        hipLaunchKernelGGL((rms_norm_kernel<T, EVEN, NV, QUANT>), dim3(p.grid), dim3(p.threads), 0, (hipStream_t)stream, a);
+        if (p.nv > NV) return rn_launch<T, W, QUANT, NV * 2>(p, a, stream);
+        hipLaunchKernelGGL((rms_norm_kernel<T, W, NV, QUANT>), dim3(p.grid), dim3(p.threads), 0, (hipStream_t)stream, a);
         return ymk_launch_status();
     }
 }
-template <typename T, bool EVEN, int NV = 1>
+template <typename T, int W, int NV = 1>
 int rn_launch_backward(const RnPlan& p, const RnBwdArgs& a, void* stream) {
-    if constexpr (NV > RN_MAX_NV_BWD(T)) return YMK_E_BADARG;
+    if constexpr (NV > (W == RN_TINY ? 1 : RN_MAX_NV_BWD(T))) return YMK_E_BADARG;
     else {
-        if (p.nv > NV) return rn_launch_backward<T, EVEN, NV * 2>(p, a, stream);
-        const size_t lds = p.threads > p.group && a.part ? (size_t)p.threads * (16 / sizeof(T)) * NV * sizeof(float) : 0;
-        hipLaunchKernelGGL((rms_norm_backward_kernel<T, EVEN, NV>), dim3(p.grid), dim3(p.threads), lds, (hipStream_t)stream, a);
+        if (p.nv > NV) return rn_launch_backward<T, W, NV * 2>(p, a, stream);
+        const size_t lds = p.threads > p.group && a.part ? (size_t)(p.threads / p.group) * a.C * sizeof(float) : 0;
+        hipLaunchKernelGGL((rms_norm_backward_kernel<T, W, NV>), dim3(p.grid), dim3(p.threads), lds, (hipStream_t)stream, a);
         return ymk_launch_status();
     }
+}
+
+template <typename T, bool QUANT>
+int rn_width(const RnPlan& p, const RnArgs& a, void* stream) {
+    constexpr int V = 16 / sizeof(T);
+    return a.C < V ? rn_launch<T, RN_TINY, QUANT>(p, a, stream) : a.C % V ? rn_launch<T, RN_RAGGED, QUANT>(p, a, stream) : rn_launch<T, RN_EVEN, QUANT>(p, a, stream);
+}
+template <typename T>
+int rn_width_backward(const RnPlan& p, const RnBwdArgs& a, void* stream) {
+    constexpr int V = 16 / sizeof(T);
+    return a.C < V ? rn_launch_backward<T, RN_TINY>(p, a, stream) : a.C % V ? rn_launch_backward<T, RN_RAGGED>(p, a, stream) : rn_launch_backward<T, RN_EVEN>(p, a, stream);
 }
 
 int rms_norm_any(bool quant, int32_t dtype, const void* x, int32_t ldx, const void* residual, int32_t ldr, void* h, int32_t ldh, void* y, int32_t ldy,
@@ -365,16 +373,10 @@ int rms_norm_any(bool quant, int32_t dtype, const void* x, int32_t ldx, const vo
     if (!weight || rn_bad(x, ldx, C, es) || (residual && (rn_bad(residual, ldr, C, es) || rn_bad(h, ldh, C, es))) || rn_bad(y, ldy, C, quant ? 1 : es) || (quant && !stat))
         return YMK_E_BADARG;
     const int V = 16 / es;
-    const bool even = C % V == 0 && ldx % V == 0 && rn_al(x, 16) && (!residual || (ldr % V == 0 && ldh % V == 0 && rn_al(residual, 16) && rn_al(h, 16))) &&
-                      ldy % V == 0 && rn_al(y, quant ? V : 16);
-    const RnPlan p = rn_plan(rows, (C + V - 1) / V, dtype == YMK_F32 ? RN_MAX_NV(float) : RN_MAX_NV(h16_t), RN_MAX_WAVES, RN_MAX_GROUPS);
+    const RnPlan p = rn_plan(rows, (C + V - 1) / V, dtype == YMK_F32 ? RN_MAX_NV(float) : RN_MAX_NV(h16_t), dtype == YMK_F32 ? RN_MAX_NV(float) / 2 : RN_MAX_NV(h16_t) / 2, RN_MAX_WAVES, RN_MAX_GROUPS);
     const RnArgs a{x, residual, h, y, stat, weight, rows, ldx, ldr, ldh, ldy, C, p.group, eps};
-    if (dtype == YMK_F32) {
-        if (quant) return even ? rn_launch<float, true, true>(p, a, stream) : rn_launch<float, false, true>(p, a, stream);
-        return even ? rn_launch<float, true, false>(p, a, stream) : rn_launch<float, false, false>(p, a, stream);
-    }
-    if (quant) return even ? rn_launch<h16_t, true, true>(p, a, stream) : rn_launch<h16_t, false, true>(p, a, stream);
-    return even ? rn_launch<h16_t, true, false>(p, a, stream) : rn_launch<h16_t, false, false>(p, a, stream);
+    if (dtype == YMK_F32) return quant ? rn_width<float, true>(p, a, stream) : rn_width<float, false>(p, a, stream);
+    return quant ? rn_width<h16_t, true>(p, a, stream) : rn_width<h16_t, false>(p, a, stream);
 }
 
 }  // namespace
@@ -403,12 +405,9 @@ extern "C" int ymk_rms_norm_backward(int32_t dtype, const void* dy, int32_t lddy
     if (dweight && rows > 0 && (!workspace || workspace_bytes < ymk_rms_norm_backward_workspace_bytes(rows, C))) return YMK_E_WORKSPACE;
     if (rows > 0) {
         const int V = 16 / es;
-        const bool even = C % V == 0 && lddy % V == 0 && ldh % V == 0 && lddx % V == 0 && rn_al(dy, 16) && rn_al(h, 16) && rn_al(dx, 16) &&
-                          (!dres || (lddr % V == 0 && rn_al(dres, 16)));
-        const RnPlan p = rn_plan(rows, (C + V - 1) / V, dtype == YMK_F32 ? RN_MAX_NV_BWD(float) : RN_MAX_NV_BWD(h16_t), (int64_t)RN_BWD_BLOCKS * 4, RN_BWD_BLOCKS);
+        const RnPlan p = rn_plan(rows, (C + V - 1) / V, dtype == YMK_F32 ? RN_MAX_NV_BWD(float) : RN_MAX_NV_BWD(h16_t), dtype == YMK_F32 ? RN_MAX_NV_BWD(float) : RN_MAX_NV_BWD(h16_t), (int64_t)RN_BWD_BLOCKS * 4, RN_BWD_BLOCKS);
         const RnBwdArgs a{dy, h, rstd, weight, dres, dx, dweight ? static_cast<float*>(workspace) : nullptr, rows, lddy, ldh, lddr, lddx, C, p.group};
-        const int rc = dtype == YMK_F32 ? (even ? rn_launch_backward<float, true>(p, a, stream) : rn_launch_backward<float, false>(p, a, stream))
-                                        : (even ? rn_launch_backward<h16_t, true>(p, a, stream) : rn_launch_backward<h16_t, false>(p, a, stream));
+        const int rc = dtype == YMK_F32 ? rn_width_backward<float>(p, a, stream) : rn_width_backward<h16_t>(p, a, stream);
         if (rc != YMK_OK || !dweight) return rc;
         hipLaunchKernelGGL(rms_norm_dweight_kernel, dim3((unsigned)((C + 15) / 16)), dim3(1024), 0, (hipStream_t)stream, static_cast<const float*>(workspace), (int)p.grid,
                            (int)C, dweight);

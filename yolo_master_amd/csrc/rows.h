@@ -1,6 +1,8 @@
 // Vector access to rows of any width and alignment, for the row-wise token kernels (csrc/rmsnorm.hip, tokens.hip).  A lane handles 16 bytes of a row at
-// a time: EVEN rows (16-byte aligned, a whole number of vectors) with aligned accesses, others with 16-byte accesses at the element's alignment, which
-// the hardware splits where they cross a line (a row of 1021 fp32 values at 16 bytes a lane instead of 4: RN_ODD).
+// a time, at the element's alignment (the hardware splits an access where it crosses a line).  The last vector of a row ends with the row: where the
+// width is no whole number of vectors it overlaps the one before it, both lanes hold the shared elements and write the same bytes.  Nothing branches on
+// the width, so all loads of a row are in flight together (with a branch for the row's end each vector was waited for by itself: 15760 x 774 fp32,
+// norm and gradients, 185 us).  Rows narrower than a vector are loaded element by element.
 #pragma once
 #include "ymk_common.h"
 
@@ -23,31 +25,28 @@ __device__ __forceinline__ u32x4 row_narrow(const float (&v)[4]) {
     return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
 }
 
-// the first n (1 .. V) of V elements at p; the others are left as they are
-template <typename T, bool EVEN, int V>
-__device__ __forceinline__ void row_load(const T* p, int n, float (&v)[V]) {
-    static_assert(V * sizeof(T) == 16, "16 bytes a lane");
-    if constexpr (EVEN) row_widen(*reinterpret_cast<const u32x4*>(p), v);
-    else if (n >= V) {
-        const u32x4 t = *reinterpret_cast<const u32x4_u*>(p);
-        row_widen(t, v);
-    }
+// 16 bytes of a row of n elements (n < V: those, with zeros behind them)
+template <typename T, bool TINY>
+__device__ __forceinline__ u32x4 row_load(const T* p, int n) {
+    if constexpr (!TINY) return *reinterpret_cast<const u32x4_u*>(p);
     else {
+        constexpr int V = 16 / sizeof(T);
+        float v[V];
 #pragma unroll
-        for (int e = 0; e < V - 1; ++e) {   // no branches: the last one again, not used
+        for (int e = 0; e < V; ++e) {
             const float t = to_f32(p[e < n ? e : n - 1]);
-            v[e] = e < n ? t : v[e];
+            v[e] = e < n ? t : 0.f;
         }
+        return row_narrow(v);
     }
 }
-template <typename T, bool EVEN, int V>
+template <typename T, bool TINY, int V>
 __device__ __forceinline__ void row_store(T* p, int n, const float (&v)[V]) {
     static_assert(V * sizeof(T) == 16, "16 bytes a lane");
-    if constexpr (EVEN) *reinterpret_cast<u32x4*>(p) = row_narrow(v);
-    else if (n >= V) *reinterpret_cast<u32x4_u*>(p) = row_narrow(v);
+    if constexpr (!TINY) *reinterpret_cast<u32x4_u*>(p) = row_narrow(v);
     else {
 #pragma unroll
-        for (int e = 0; e < V - 1; ++e)
+        for (int e = 0; e < V; ++e)
             if (e < n) from_f32(p[e], v[e]);
     }
 }

@@ -213,7 +213,7 @@ struct CombineArgs {
 template <typename T, int V>
 __device__ __forceinline__ void tk_load(const T* p, float (&v)[V]) {
     if constexpr (V == 1) v[0] = to_f32(*p);
-    else row_load<T, false>(p, V, v);
+    else row_widen(row_load<T, false>(p, V), v);
 }
 template <typename T, int V>
 __device__ __forceinline__ void tk_store(T* p, const float (&v)[V]) {
