@@ -8,6 +8,7 @@ synchronises.  torch is used for memory and streams only — all arithmetic is i
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -702,8 +703,6 @@ def _tensor_bytes(obj) -> int:
 def _timed(family: str, flops=None):
     """Per-call HIP-event timing of a config-5 op under `family` (bench.py's roofline leg; inactive unless TIMER.start() was called).
     Algorithmic bytes = every tensor argument once + the result once; flops from the op's shapes where it has a contraction."""
-    import functools
-
     def wrap(fn):
         @functools.wraps(fn)
         def run(*a, **kw):
@@ -1199,9 +1198,23 @@ _ROW_DT = {**DT, E4M3: _lib.YMK_E4M3}
 _ROW_ACT = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "sigmoid": _lib.ACT_SIGMOID}
 
 
+def _lib_for(dtype):
+    """The library of a dtype, without the router's lookups: libymk_f16.so for float16, libymk.so for everything else."""
+    if type(lib) is not _LibRouter:   # another library bound in its place
+        if dtype in H16:
+            _TLS.fmt = dtype
+        return lib
+    if dtype is torch.float16:
+        return _lib._lib_f16 or _lib.load_f16()
+    return _lib._lib or _lib.load()
+
+
 def _rows(t: torch.Tensor, what: str):
     """(rows, C, ld) of a row view."""
-    shape, strides = t.shape, t.stride()
+    shape = t.shape
+    if len(shape) == 2 and t.is_contiguous() and shape[1]:
+        return shape[0], shape[1], shape[1]
+    strides = t.stride()
     if len(shape) == 2:
         M, Cc = shape
         ld, dense = strides
@@ -1226,16 +1239,18 @@ def _rows(t: torch.Tensor, what: str):
     return M, Cc, ld
 
 
-def _here(what: str, first: torch.Tensor, *others) -> None:
-    """All operands on one GPU, and that the current one (the call goes to its current stream)."""
+def _here(what: str, first: torch.Tensor, *others):
+    """All operands on one GPU, and that the current one; its current stream, where the call goes."""
     dev = first.get_device()
-    if dev < 0:
-        require_gpu(first, what)
-    elif dev != torch.cuda.current_device():
-        raise ValueError(f"{what}: operands on {first.device}, current device cuda:{torch.cuda.current_device()}")
     for t in others:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{what}: operands on {first.device} and {t.device}")
+    if dev < 0:
+        require_gpu(first, what)
+        return _stream()
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{what}: operands on {first.device}, current device cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _fp32_vec(t, shape, what: str, name: str) -> None:
@@ -1245,9 +1260,10 @@ def _fp32_vec(t, shape, what: str, name: str) -> None:
 
 def _like(t, x, what: str, name: str):
     """t's row stride; t is a view of x's shape and dtype."""
-    if t.dtype is not x.dtype or t.shape != x.shape:
+    shape = x.shape
+    if t.dtype is not x.dtype or t.shape != shape:
         raise ValueError(f"{what}: {name} is {t.dtype} {list(t.shape)}, expected {x.dtype} {list(x.shape)}")
-    return _rows(t, what)[2]
+    return shape[-1] if t.is_contiguous() else _rows(t, what)[2]
 
 
 def _ptr(t):
@@ -1266,38 +1282,39 @@ def _new_stat(x, M: int, fp32):
 
 
 def _norm_args(what, x, weight, residual, residual_out):
-    if x.dtype not in DT:
-        raise ValueError(f"{what}: dtype {x.dtype}")
-    _here(what, x, weight, residual, residual_out)
+    dt = x.dtype
+    if dt not in DT:
+        raise ValueError(f"{what}: dtype {dt}")
+    stream = _here(what, x, weight, residual, residual_out)
     M, Cc, ldx = _rows(x, what)
     if not 1 <= Cc <= _lib.NORM_MAX_C:
         raise ValueError(f"{what}: {Cc} channels (1 .. {_lib.NORM_MAX_C})")
     _fp32_vec(weight, (Cc,), what, "weight")
-    use_format(x.dtype)
     if residual is None:
         if residual_out is not None:
             raise ValueError(f"{what}: residual_out without a residual")
-        return M, Cc, ldx, 0, x, 0
+        return stream, M, Cc, ldx, 0, x, 0
     ldr = _like(residual, x, what, "residual")
     if residual_out is None:
-        return M, Cc, ldx, ldr, _new(x, x.dtype), Cc
+        return stream, M, Cc, ldx, ldr, _new(x, dt), Cc
     ldh = _like(residual_out, x, what, "residual_out")
     for t, ld in ((x, ldx), (residual, ldr)):   # in place is fine, row by row; a shifted view is not
         a, b = t.data_ptr(), residual_out.data_ptr()
         span = ((M - 1) * max(ld, ldh) + Cc) * x.element_size()
         if M and not (a == b and (ld == ldh or M == 1)) and abs(a - b) < span:
             raise ValueError(f"{what}: residual_out overlaps an input without being it")
-    return M, Cc, ldx, ldr, residual_out, ldh
+    return stream, M, Cc, ldx, ldr, residual_out, ldh
 
 
 @_timed("rms_norm")
 def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
     """h = x + residual (rounded to x's dtype; h is x without a residual), y = h / sqrt(mean(h^2) + eps) * weight.  Returns (y, h, rstd); rstd
     fp32, one a row, is what rms_norm_backward takes.  residual_out: where h goes (x or residual themselves, or a tensor apart from them)."""
-    M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm", x, weight, residual, residual_out)
-    y, rstd = _new(x, x.dtype), _new_stat(x, M, weight)
-    check(lib.ymk_rms_norm(DT[x.dtype], x.data_ptr(), ldx, _ptr(residual), ldr, None if residual is None else h.data_ptr(), ldh, y.data_ptr(), Cc, rstd.data_ptr(),
-                           M, Cc, weight.data_ptr(), eps, _stream()), "rms_norm")
+    stream, M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm", x, weight, residual, residual_out)
+    dt = x.dtype
+    y, rstd = _new(x, dt), _new_stat(x, M, weight)
+    check(_lib_for(dt).ymk_rms_norm(DT[dt], x.data_ptr(), ldx, _ptr(residual), ldr, None if residual is None else h.data_ptr(), ldh, y.data_ptr(), Cc,
+                                    rstd.data_ptr(), M, Cc, weight.data_ptr(), eps, stream), "rms_norm")
     return y, h, rstd
 
 
@@ -1305,11 +1322,17 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
 def rms_norm_quant(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
     """The same norm with an 8-bit output: (q, scale, h), q e4m3 of x's shape and scale fp32 per row with y = q * scale, max |q| = 448
     (an all-zero row: scale 1; a row with a NaN or an infinity: all NaN)."""
-    M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm_quant", x, weight, residual, residual_out)
+    stream, M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm_quant", x, weight, residual, residual_out)
+    dt = x.dtype
     q, scale = _new(x, E4M3), _new_stat(x, M, weight)
-    check(lib.ymk_rms_norm_quant(DT[x.dtype], x.data_ptr(), ldx, _ptr(residual), ldr, None if residual is None else h.data_ptr(), ldh, q.data_ptr(), Cc,
-                                 scale.data_ptr(), M, Cc, weight.data_ptr(), eps, _stream()), "rms_norm_quant")
+    check(_lib_for(dt).ymk_rms_norm_quant(DT[dt], x.data_ptr(), ldx, _ptr(residual), ldr, None if residual is None else h.data_ptr(), ldh, q.data_ptr(), Cc,
+                                          scale.data_ptr(), M, Cc, weight.data_ptr(), eps, stream), "rms_norm_quant")
     return q, scale, h
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(M: int, Cc: int) -> int:
+    return _lib.load().ymk_rms_norm_backward_workspace_bytes(M, Cc) // 4
 
 
 @_timed("rms_norm")
@@ -1317,9 +1340,10 @@ def rms_norm_backward(dy, h, weight, rstd, dres=None, need_dweight: bool = True)
     """Gradient of rms_norm: (dx, dweight) from dy and the h, rstd it returned; dres is the gradient that reaches h by its other use (the residual
     stream).  dx is the gradient of x and of residual alike; dweight fp32 (None unless wanted)."""
     what = "rms_norm_backward"
-    if h.dtype not in DT:
-        raise ValueError(f"{what}: dtype {h.dtype}")
-    _here(what, h, dy, weight, rstd, dres)
+    dt = h.dtype
+    if dt not in DT:
+        raise ValueError(f"{what}: dtype {dt}")
+    stream = _here(what, h, dy, weight, rstd, dres)
     M, Cc, ldh = _rows(h, what)
     if not 1 <= Cc <= _lib.NORM_MAX_C:
         raise ValueError(f"{what}: {Cc} channels (1 .. {_lib.NORM_MAX_C})")
@@ -1327,15 +1351,14 @@ def rms_norm_backward(dy, h, weight, rstd, dres=None, need_dweight: bool = True)
     _fp32_vec(rstd, h.shape[:-1], what, "rstd")
     lddy = _like(dy, h, what, "dy")
     lddr = _like(dres, h, what, "dres") if dres is not None else 0
-    use_format(h.dtype)
-    dx = _new(h, h.dtype)
+    dx = _new(h, dt)
     dweight = ws = None
-    nbytes = 0
+    n = 0
     if need_dweight:
-        nbytes = lib.ymk_rms_norm_backward_workspace_bytes(M, Cc)
-        dweight, ws = weight.new_empty(Cc), weight.new_empty(nbytes // 4)
-    check(lib.ymk_rms_norm_backward(DT[h.dtype], dy.data_ptr(), lddy, h.data_ptr(), ldh, rstd.data_ptr(), weight.data_ptr(), _ptr(dres), lddr, dx.data_ptr(), Cc,
-                                    _ptr(dweight), M, Cc, _ptr(ws), nbytes, _stream()), what)
+        n = _norm_workspace(M, Cc)
+        dweight, ws = weight.new_empty(Cc), weight.new_empty(n)
+    check(_lib_for(dt).ymk_rms_norm_backward(DT[dt], dy.data_ptr(), lddy, h.data_ptr(), ldh, rstd.data_ptr(), weight.data_ptr(), _ptr(dres), lddr, dx.data_ptr(), Cc,
+                                             _ptr(dweight), M, Cc, _ptr(ws), 4 * n, stream), what)
     return dx, dweight
 
 
@@ -1349,21 +1372,26 @@ class TokenPlan(NamedTuple):
     experts: int
 
 
+@functools.lru_cache(maxsize=256)
+def _sort_workspace(T: int, K: int, experts: int) -> int:
+    return _lib.load().ymk_token_sort_workspace_bytes(T, K, experts) // 4
+
+
 @_timed("token_sort")
 def token_sort(idx, experts: int) -> TokenPlan:
     """Stable sort of the pairs idx [tokens, top_k] (int32 or int64; values outside [0, experts) have no expert) by expert."""
     if idx.dim() != 2 or idx.dtype not in (torch.int32, torch.int64) or not idx.is_contiguous():
         raise ValueError("token_sort: idx is a contiguous int32 or int64 [tokens, top_k] tensor")
-    _here("token_sort", idx)
+    stream = _here("token_sort", idx)
     T, K = idx.shape
     if not 1 <= K <= _lib.TOKEN_MAX_K or not 1 <= experts <= _lib.TOKEN_MAX_E or T * K >= 1 << 30:
         raise ValueError(f"token_sort: top_k {K} (1 .. {_lib.TOKEN_MAX_K}), {experts} experts (1 .. {_lib.TOKEN_MAX_E}), {T} tokens")
     row = torch.empty_like(idx, dtype=torch.int32)
     offsets, src = row.new_empty(experts + 1), row.new_empty(T * K)
-    nbytes = lib.ymk_token_sort_workspace_bytes(T, K, experts)
-    ws = row.new_empty(nbytes // 4) if nbytes else None
-    check(lib.ymk_token_sort(idx.data_ptr(), idx.element_size(), T, K, experts, offsets.data_ptr(), src.data_ptr(), row.data_ptr(), _ptr(ws), nbytes, _stream()),
-          "token_sort")
+    n = _sort_workspace(T, K, experts)
+    ws = row.new_empty(n) if n else None
+    check(_lib_for(torch.int32).ymk_token_sort(idx.data_ptr(), idx.element_size(), T, K, experts, offsets.data_ptr(), src.data_ptr(), row.data_ptr(), _ptr(ws), 4 * n,
+                                               stream), "token_sort")
     return TokenPlan(offsets, src, row, experts)
 
 
@@ -1380,7 +1408,7 @@ def _planned(what, plan, t, rows=None):
 def token_dispatch(x, plan: TokenPlan, scale=None):
     """xs[plan.row[t][k]] = x[t], any element type; with scale (fp32 [tokens], of an 8-bit x) -> (xs, xs_scale).  Rows behind the last expert's are
     not written."""
-    _here("token_dispatch", x, plan.row, scale)
+    stream = _here("token_dispatch", x, plan.row, scale)
     T, K, Cc, ldx = _planned("token_dispatch", plan, x)
     es = x.element_size()
     xs = x.new_empty(T * K, Cc)
@@ -1389,21 +1417,20 @@ def token_dispatch(x, plan: TokenPlan, scale=None):
         if scale.numel() != T or scale.dtype != torch.float32 or not scale.is_contiguous():
             raise ValueError(f"token_dispatch: scale is contiguous fp32, one a token ({T})")
         xs_scale = scale.new_empty(T * K)
-    check(lib.ymk_token_dispatch(x.data_ptr(), ldx * es, Cc * es, _ptr(scale), xs.data_ptr(), Cc * es, _ptr(xs_scale), plan.row.data_ptr(), T, K, _stream()),
-          "token_dispatch")
+    check(_lib_for(x.dtype).ymk_token_dispatch(x.data_ptr(), ldx * es, Cc * es, _ptr(scale), xs.data_ptr(), Cc * es, _ptr(xs_scale), plan.row.data_ptr(), T, K,
+                                               stream), "token_dispatch")
     return xs if scale is None else (xs, xs_scale)
 
 
 def _combine(what, ys, plan, w):
     if ys.dtype not in DT:
         raise ValueError(f"{what}: dtype {ys.dtype}")
-    _here(what, ys, plan.row, w)
+    stream = _here(what, ys, plan.row, w)
     T, K, Cc, ldys = _planned(what, plan, ys, rows=True)
     if w is not None:
         _fp32_vec(w, (T, K), what, "w")
-    use_format(ys.dtype)
     y = ys.new_empty(T, Cc)
-    check(lib.ymk_token_combine(DT[ys.dtype], ys.data_ptr(), ldys, plan.row.data_ptr(), _ptr(w), y.data_ptr(), Cc, T, K, Cc, _stream()), what)
+    check(_lib_for(ys.dtype).ymk_token_combine(DT[ys.dtype], ys.data_ptr(), ldys, plan.row.data_ptr(), _ptr(w), y.data_ptr(), Cc, T, K, Cc, stream), what)
     return y
 
 
@@ -1428,16 +1455,15 @@ def token_combine_backward(dy, ys, plan: TokenPlan, w):
     what = "token_combine_backward"
     if ys.dtype not in DT or dy.dtype != ys.dtype:
         raise ValueError(f"{what}: dtypes {dy.dtype}, {ys.dtype}")
-    _here(what, ys, dy, plan.row, w)
+    stream = _here(what, ys, dy, plan.row, w)
     T, K, Cc, ldys = _planned(what, plan, ys, rows=True)
     _, _, Cd, lddy = _planned(what, plan, dy)
     if Cd != Cc:
         raise ValueError(f"{what}: dy has {Cd} channels, ys {Cc}")
     _fp32_vec(w, (T, K), what, "w")
-    use_format(ys.dtype)
     dys, dw = ys.new_empty(T * K, Cc), torch.empty_like(w)
-    check(lib.ymk_token_combine_backward(DT[ys.dtype], dy.data_ptr(), lddy, ys.data_ptr(), ldys, plan.row.data_ptr(), w.data_ptr(), dys.data_ptr(), Cc, dw.data_ptr(),
-                                         T, K, Cc, _stream()), what)
+    check(_lib_for(ys.dtype).ymk_token_combine_backward(DT[ys.dtype], dy.data_ptr(), lddy, ys.data_ptr(), ldys, plan.row.data_ptr(), w.data_ptr(), dys.data_ptr(), Cc,
+                                                        dw.data_ptr(), T, K, Cc, stream), what)
     return dys, dw
 
 
@@ -1451,8 +1477,6 @@ def _expert_args(what, x, w, offsets):
         raise ValueError(f"{what}: offsets is a contiguous int32 [{E + 1}] tensor")
     if E > _lib.TOKEN_MAX_E:
         raise ValueError(f"{what}: {E} experts (at most {_lib.TOKEN_MAX_E})")
-    if x.dtype in H16:
-        use_format(x.dtype)
     return E, Cout, Cin
 
 
@@ -1460,7 +1484,8 @@ def _expert_rows(what, t, Cc):
     M, c, ld = _rows(t, what)
     if c != Cc:
         raise ValueError(f"{what}: rows of {c} channels, expected {Cc}")
-    if t.data_ptr() % 16 or ld * t.element_size() % 16 or Cc * t.element_size() % 16:
+    es = t.element_size()
+    if (t.data_ptr() | ld * es | Cc * es) & 15:
         raise ValueError(f"{what}: rows of {Cc} x {t.dtype} at a stride of {ld} are not 16-byte aligned")
     return M, ld
 
@@ -1472,7 +1497,7 @@ def expert_linear(x, w, offsets, bias=None, act=None, x_scale=None, w_scale=None
     [experts, Cout], act None | "silu" | "gelu" | "sigmoid".  The output has x's dtype; e4m3 rows give out_dtype (bfloat16 unless said)."""
     what = "expert_linear"
     E, Cout, Cin = _expert_args(what, x, w, offsets)
-    _here(what, x, w, offsets, bias, x_scale, w_scale)
+    stream = _here(what, x, w, offsets, bias, x_scale, w_scale)
     M, ldx = _expert_rows(what, x, Cin)
     odt = x.dtype
     if x.dtype == E4M3:
@@ -1483,8 +1508,6 @@ def expert_linear(x, w, offsets, bias=None, act=None, x_scale=None, w_scale=None
             raise ValueError(f"{what}: e4m3 operands need x_scale and w_scale")
         _fp32_vec(x_scale, (M,), what, "x_scale")
         _fp32_vec(w_scale, (E, Cout), what, "w_scale")
-        if odt in H16:
-            use_format(odt)
     elif x_scale is not None or w_scale is not None or out_dtype not in (None, x.dtype):
         raise ValueError(f"{what}: scales and another out_dtype belong to e4m3 operands")
     if Cout % (8 if odt != torch.float32 or x.dtype == E4M3 else 4) or w.data_ptr() % 16:
@@ -1494,8 +1517,8 @@ def expert_linear(x, w, offsets, bias=None, act=None, x_scale=None, w_scale=None
     if act not in _ROW_ACT:
         raise ValueError(f"{what}: act {act!r}")
     y = x.new_empty((M, Cout), dtype=odt)
-    check(lib.ymk_expert_linear(_ROW_DT[x.dtype], DT[odt], x.data_ptr(), ldx, _ptr(x_scale), w.data_ptr(), _ptr(w_scale), _ptr(bias), offsets.data_ptr(), y.data_ptr(),
-                                Cout, M, E, Cin, Cout, _ROW_ACT[act], _stream()), what)
+    check(_lib_for(odt).ymk_expert_linear(_ROW_DT[x.dtype], DT[odt], x.data_ptr(), ldx, _ptr(x_scale), w.data_ptr(), _ptr(w_scale), _ptr(bias), offsets.data_ptr(),
+                                          y.data_ptr(), Cout, M, E, Cin, Cout, _ROW_ACT[act], stream), what)
     return y
 
 
@@ -1511,7 +1534,8 @@ def expert_linear_backward(dy, x, w, offsets, need_dx: bool = True, need_dw: boo
         raise ValueError(f"{what}: dw_dtype {dw_dtype}")
     if need_db and not need_dw:
         raise ValueError(f"{what}: db comes with dw")
-    _here(what, x, dy, w, offsets)
+    stream = _here(what, x, dy, w, offsets)
+    h = _lib_for(x.dtype)
     M, ldx = _expert_rows(what, x, Cin)
     Md, lddy = _expert_rows(what, dy, Cout)
     if Md != M or w.data_ptr() % 16:
@@ -1519,11 +1543,11 @@ def expert_linear_backward(dy, x, w, offsets, need_dx: bool = True, need_dw: boo
     dx = dw = db = None
     if need_dx:
         dx = x.new_empty(M, Cin)
-        check(lib.ymk_expert_linear_dx(DT[x.dtype], dy.data_ptr(), lddy, w.data_ptr(), offsets.data_ptr(), dx.data_ptr(), Cin, M, E, Cin, Cout, _stream()),
+        check(h.ymk_expert_linear_dx(DT[x.dtype], dy.data_ptr(), lddy, w.data_ptr(), offsets.data_ptr(), dx.data_ptr(), Cin, M, E, Cin, Cout, stream),
               "expert_linear_dx")
     if need_dw:
         dw = torch.empty_like(w, dtype=dw_dtype or x.dtype)
         db = x.new_empty((E, Cout), dtype=torch.float32) if need_db else None
-        check(lib.ymk_expert_linear_dw(DT[x.dtype], DT[dw.dtype], dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(), dw.data_ptr(), _ptr(db), M, E, Cin, Cout,
-                                       _stream()), "expert_linear_dw")
+        check(h.ymk_expert_linear_dw(DT[x.dtype], DT[dw.dtype], dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(), dw.data_ptr(), _ptr(db), M, E, Cin, Cout,
+                                     stream), "expert_linear_dw")
     return dx, dw, db
