@@ -236,3 +236,23 @@ def test_large_offsets(ops):
             tc.close(dx[r], want, want.abs() * 2.0**-8 + 1e-4, "dx")
         want = dz[off[e]:off[e + 1]].double().t() @ xs[off[e]:off[e + 1], :8].double()
         tc.close(dw[e][:, :8], want, want.abs() * 2.0**-8 + (off[e + 1] - off[e]) * 8 * 2.0**-24, "dw")
+
+
+def test_product_wide_tiles_by_the_rule(ops):
+    """More tiles of 256 than CUs, by the rule: ragged experts, an empty one, more experts than a wave has lanes."""
+    for counts, Cin, Cout in (([3000, 0, 2100, 4097, 700, 6000], 200, 2576), ([250] * 70, 64, 1032)):
+        tc.check_product(ops, torch.bfloat16, (counts, 3, Cin, Cout, "silu", 8), DEV)
+        g = torch.Generator(device=DEV).manual_seed(3)
+        off = tc.make_offsets(counts)
+        R, E = int(off[-1]), len(counts)
+        x, w, dy = (torch.randn(*s, generator=g, device=DEV) for s in ((R, Cin), (E, Cout, Cin), (R, Cout)))
+        for dt in (torch.bfloat16, torch.float32):
+            xt, wt, dt_ = x.to(dt), (w * Cin**-0.5).to(dt), dy.to(dt)
+            y = ops.expert_linear(xt, wt, off.to(DEV))
+            dx, dw, db = ops.expert_linear_backward(dt_, xt, wt, off.to(DEV))
+            for e in range(E):
+                s = slice(int(off[e]), int(off[e + 1]))
+                a, b, d = xt[s].double(), wt[e].double(), dt_[s].double()
+                for got, want, mag, n in ((y[s], a @ b.t(), a.abs() @ b.abs().t(), Cin), (dx[s], d @ b, d.abs() @ b.abs(), Cout), (dw[e], d.t() @ a, d.abs().t() @ a.abs(), len(a)),
+                                          (db[e], d.sum(0), d.abs().sum(0), len(a))):
+                    tc.close(got, want, mag * ((n + 8) * tc.U) + want.abs() * tc.half(got.dtype), f"{dt} expert {e}")

@@ -117,7 +117,7 @@ def test_product_at_every_tile(tile, libs):
         "h = C.CDLL(str(build.build()))\n"
         "for name, (res, args) in _lib.SYMBOLS_TOKENS.items(): fn = getattr(h, name); fn.restype, fn.argtypes = res, args\n"
         "ops.lib, ops._stream, ops.require_gpu = h, lambda: None, lambda t, what='': None\n"
-        "for c in (([130, 0, 1, 37], 3, 80, 144, 'gelu', 0), ([5, 129], 0, 208, 16, 'sigmoid', 0)):\n"
+        "for c in (([130, 0, 1, 37], 3, 80, 144, 'gelu', 0), ([5, 129], 0, 208, 16, 'sigmoid', 0), ([3, 0, 200, 1, 2, 7, 0, 1, 5, 9, 1, 1, 4, 260], 2, 48, 40, None, 0)):\n"
         "    for d in (torch.float32, torch.bfloat16): tc.check_product(ops, d, c); tc.check_product_gradient(ops, d, c)\n"
         "    tc.check_product_exact(ops, c)\n"
         "    tc.check_product(ops, torch.float8_e4m3fn, c, out_dtype=torch.float32)\n")

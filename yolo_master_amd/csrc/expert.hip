@@ -116,11 +116,12 @@ __device__ __forceinline__ void ex_load_lds(const ExBuffer& b, char* dst, unsign
 typedef u32x4 ExBuffer;
 __device__ __forceinline__ ExBuffer ex_buffer(const char* p) {
     const uint64_t a = reinterpret_cast<uint64_t>(p);
-    return ExBuffer{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
+    ExBuffer b{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
+    asm volatile("s_nop 4" : "+s"(b));   // a scalar register that a vector instruction has written may be read by a transfer five wait states later
+    return b;
 }
 __device__ __forceinline__ void ex_load_lds(const ExBuffer& b, char* dst, unsigned voff) {
-    // five wait states: M0 written by the scalar unit needs one, a scalar register written by a vector instruction (the buffer's) five
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"((uint32_t)(uintptr_t)(glds_lptr)dst), "v"(voff), "s"(b) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"((uint32_t)(uintptr_t)(glds_lptr)dst), "v"(voff), "s"(b) : "memory", "m0");   // M0 needs one wait state
 }
 #endif
 
