@@ -29,7 +29,7 @@ int ymk_rms_norm(int32_t dtype, const void* x, int32_t ldx, const void* residual
                  float* rstd, int64_t rows, int32_t C, const float* weight, float eps, void* stream);
 
 /* The same norm with an 8-bit output: scale[row] = max|y| / 448 and q = y / scale in e4m3 (round to nearest even), taken from the
- * unrounded y.  A row whose largest magnitude is below 448 * 2^-126 (an all-zero row) has scale 1 and zero codes; a row with a NaN or
+ * unrounded y.  A row whose largest magnitude is below 448 * 2^-126 (an all-zero row, eps > 0) has scale 1 and zero codes; a row with a NaN or
  * an infinity has scale NaN and NaN codes.  ldq in bytes. */
 int ymk_rms_norm_quant(int32_t dtype, const void* x, int32_t ldx, const void* residual, int32_t ldr, void* h, int32_t ldh, void* q,
                        int32_t ldq, float* scale, int64_t rows, int32_t C, const float* weight, float eps, void* stream);
@@ -51,7 +51,8 @@ int ymk_token_sort(const void* idx, int32_t idx_bytes, int64_t tokens, int32_t t
                    int32_t* row, void* workspace, size_t workspace_bytes, void* stream);
 
 /* xs[row[t][k]] = x[t], byte for byte (any element type): row_bytes of a row, strides in bytes; with scale fp32 [tokens] (may be NULL)
- * also xs_scale[row[t][k]] = scale[t].  Rows behind the last one are left as they were. */
+ * also xs_scale[row[t][k]] = scale[t].  Rows behind the last one are left as they were.  Here and below a row outside [0, tokens * top_k) is
+ * no row. */
 int ymk_token_dispatch(const void* x, int64_t ldx_bytes, int64_t row_bytes, const float* scale, void* xs, int64_t ldxs_bytes,
                        float* xs_scale, const int32_t* row, int64_t tokens, int32_t top_k, void* stream);
 
@@ -70,7 +71,7 @@ int ymk_token_combine_backward(int32_t dtype, const void* dy, int32_t lddy, cons
  * dtype YMK_F32 | YMK_H16, out_dtype the same; or YMK_E4M3 (x and W in 8 bits, W[e][o] standing for W * w_scale[e][o], x[r] for
  * x * x_scale[r], both scales fp32 and required) with out_dtype YMK_F32 | YMK_H16.  Products are added in 32 bits and the sum (scaled,
  * with bias and activation) is rounded once; of 8-bit products the matrix instruction adds 16 at a time at the largest one's exponent, 13
- * bits deep, and those sums in 32 bits.  offsets: device int32 [E + 1], ascending, within [0, rows] (values outside are clamped:
+ * bits deep, and those sums in 32 bits.  rows < 2^26.  offsets: device int32 [E + 1], ascending, within [0, rows] (values outside are clamped:
  * no access leaves the tensors); rows outside every expert are left as they were.  Cin and Cout in multiples of 16 bytes of their
  * elements (4 fp32, 8 16-bit, 16 8-bit; Cout of 8 for YMK_E4M3), all pointers and row strides 16-byte aligned, strides below 2^23 bytes. */
 int ymk_expert_linear(int32_t dtype, int32_t out_dtype, const void* x, int32_t ldx, const float* x_scale, const void* w, const float* w_scale,

@@ -51,6 +51,10 @@ def test_moves(ops, dtype, case):
     tc.check_moves(ops, dtype, case, DEV)
 
 
+def test_plans_of_ones_own(ops):
+    tc.check_plans_of_ones_own(ops, DEV)
+
+
 def test_dispatch_8bit(ops):
     tc.check_dispatch_8bit(ops, DEV)
 

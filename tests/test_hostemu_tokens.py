@@ -73,6 +73,10 @@ def test_moves(ops, dtype, case):
     tc.check_moves(ops, dtype, case)
 
 
+def test_plans_of_ones_own(ops):
+    tc.check_plans_of_ones_own(ops)
+
+
 def test_dispatch_8bit(ops):
     tc.check_dispatch_8bit(ops)
 

@@ -164,7 +164,7 @@ def check_sort(ops, case, dev="cpu"):
 
 
 # tokens, top_k, experts, channels, row padding, share without an expert
-MOVES = [(1, 1, 2, 8, 0, 0.0), (7, 2, 3, 40, 8, 0.3), (33, 3, 5, 37, 0, 0.2), (16, 16, 20, 24, 4, 0.1), (5, 2, 4, 1, 0, 0.0), (130, 2, 4, 264, 0, 0.5), (4, 4, 4, 16, 0, 1.0), (3, 2, 4, 520, 0, 0.0)]
+MOVES = [(0, 2, 4, 8, 0, 0.0), (1, 1, 2, 8, 0, 0.0), (7, 2, 3, 40, 8, 0.3), (33, 3, 5, 37, 0, 0.2), (16, 16, 20, 24, 4, 0.1), (5, 2, 4, 1, 0, 0.0), (130, 2, 4, 264, 0, 0.5), (4, 4, 4, 16, 0, 1.0), (3, 2, 4, 520, 0, 0.0)]
 
 
 def check_moves(ops, dtype, case, dev="cpu"):
@@ -182,6 +182,10 @@ def check_moves(ops, dtype, case, dev="cpu"):
     # rows behind the last expert's, and the padding, stay as they were
     buf = torch.full((T * K, C + 3), 7.0, dtype=dtype, device=dev)
     es = buf.element_size()
+    if T == 0:
+        assert ops.token_combine(rows_of(g, 0, C, dtype, 0, dev), plan, torch.zeros(0, K, device=dev)).shape == (0, C)
+        assert ops.token_combine_backward(x, xs, plan, torch.zeros(0, K, device=dev))[1].shape == (0, K)
+        return
     rc = ops.lib.ymk_token_dispatch(C_.c_void_p(x.data_ptr()), (C + pad) * es if T > 1 else C * es, C * es, None, C_.c_void_p(buf.data_ptr()), (C + 3) * es, None,
                                     C_.c_void_p(plan.row.data_ptr()), T, K, ops._stream())
     assert rc == 0 and torch.equal(buf[:n, :C].cpu(), x.cpu()[tok]) and bool((buf[n:] == 7).all()) and bool((buf[:, C:] == 7).all())
@@ -217,7 +221,7 @@ def check_dispatch_8bit(ops, dev="cpu"):
 
 # --------------------------------------------------------------------------------------------------------------- product
 # rows per expert, rows behind them, Cin, Cout, activation, row padding of x
-PRODUCTS = [([1], 0, 16, 16, None, 0), ([0, 3, 0, 5], 2, 64, 48, "silu", 16), ([130, 0, 1, 37], 3, 80, 144, "gelu", 0), ([5, 129], 0, 208, 16, "sigmoid", 0),
+PRODUCTS = [([0, 0], 0, 16, 24, "silu", 0), ([1], 0, 16, 16, None, 0), ([0, 3, 0, 5], 2, 64, 48, "silu", 16), ([130, 0, 1, 37], 3, 80, 144, "gelu", 0), ([5, 129], 0, 208, 16, "sigmoid", 0),
             ([0, 0], 4, 32, 32, None, 0), ([64, 20], 0, 144, 272, None, 16)]
 
 
@@ -392,3 +396,21 @@ def check_block_gradient(ops, dev="cpu", T=11, C=32, H=48, E=3, K=2):
     for got, want, what in ((out, ref.detach(), "out"), (dx, x64.grad, "dx"), (dnorm, q["norm"].grad, "dnorm"), (dgate, gate64.grad, "dgate"), (dw1, q["w1"].grad, "dw1"),
                             (db1, q["b1"].grad, "db1"), (dw2, q["w2"].grad, "dw2"), (db2, q["b2"].grad, "db2")):
         close(got, want, torch.full_like(want, 5 * 128 * 40 * U * float(want.abs().max())), what)
+
+
+def check_plans_of_ones_own(ops, dev="cpu"):
+    """A plan with rows outside the pairs (it did not come from token_sort): nothing is read or written there, those pairs have no row."""
+    T, K, C = 6, 2, 40
+    row = torch.tensor([[0, 12], [1, -1], [-7, 2**31 - 1], [3, 4], [-2**31, 5], [11, 2]], dtype=torch.int32)
+    good = (row >= 0) & (row < T * K)
+    plan = ops.TokenPlan(torch.zeros(3, dtype=torch.int32, device=dev), torch.zeros(T * K, dtype=torch.int32, device=dev), row.to(dev), 2)
+    g = gen(8)
+    x, ys, w = rows_of(g, T, C, torch.float32, 0, dev), rows_of(g, T * K, C, torch.float32, 0, dev), torch.rand(T, K, generator=g).to(dev)
+    xs = ops.token_dispatch(x, plan)
+    at = row[good].long()
+    assert torch.equal(xs.cpu()[at], x.cpu()[:, None].expand(T, K, C)[good])
+    part = torch.where(good[..., None], ys.cpu().double()[row.clamp(0, T * K - 1).long()], 0.0)
+    close(ops.token_combine(ys, plan, w), (part * w.cpu().double()[..., None]).sum(1), torch.full((T, C), 1e-5), "combine")
+    dys, dw = ops.token_combine_backward(x, ys, plan, w)
+    close(dw, (part * x.cpu().double()[:, None]).sum(-1), torch.full((T, K), 1e-4), "dw")
+    close(dys.cpu()[at], (w.cpu()[..., None] * x.cpu()[:, None])[good].double(), torch.full((len(at), C), 1e-6), "dys")

@@ -245,6 +245,7 @@ __device__ __forceinline__ bool ex_find(const ExArgs& a, ExTile& t) {
         incl[c] = total + s;
         total += __builtin_amdgcn_readlane(s, 63);
     }
+    if ((int64_t)total * nt > 0x7ffffff0) return false;   // offsets that are no offsets: the host's grid holds every tile of ascending ones
     const int all = total * nt, per = (all + 7) / 8, slot = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + slot;
     if (slot >= per || id >= all) return false;
     const int g = id / (GM * nt), size = min(GM, total - g * GM), r = id - g * (GM * nt), m = g * GM + r % size;
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : TILE == 128 ? 2 : 4) void ex
 template <auto Kernel>
 int ex_launch(const ExArgs& a, int64_t blocks, size_t lds, void* stream) {
     if (blocks <= 0) return YMK_OK;
-    if (blocks > 0x7fffffff) return YMK_E_BADARG;
+    if (blocks > 0x7ffffff0) return YMK_E_BADARG;
     static YmkOncePerDevice once;
     if (once.need()) {
         if (hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return YMK_E_LAUNCH;
@@ -648,7 +649,7 @@ int ex_rows(const ExArgs& a, void* stream) {
     if constexpr (NKC) {
         if (tile == 16) {
             const int64_t blocks = ex_blocks(a.rows, a.E, a.N, 16, EX_FEW_N);
-            if (blocks > 0x7fffffff) return YMK_E_BADARG;
+            if (blocks > 0x7ffffff0) return YMK_E_BADARG;
             hipLaunchKernelGGL((expert_few_rows_kernel<T, TO>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
             return ymk_launch_status();
         }
@@ -674,7 +675,7 @@ int ex_dw(const ExArgs& a, void* stream) {
 inline bool ex_bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15); }
 inline bool ex_bad_ld(int64_t ld, int64_t C, int es) { return ld < C || ld * es % 16 || ld * es >= (1 << 23); }
 inline bool ex_bad_sizes(int64_t rows, int32_t E, int32_t Cin, int32_t Cout) {
-    return rows < 0 || rows >= (1ll << 30) || E < 1 || E > YMK_TOKEN_MAX_E || Cin < 1 || Cout < 1;
+    return rows < 0 || rows >= (1ll << 26) || E < 1 || E > YMK_TOKEN_MAX_E || Cin < 1 || Cout < 1;
 }
 
 }  // namespace
@@ -684,10 +685,11 @@ extern "C" int ymk_expert_linear(int32_t dtype, int32_t out_dtype, const void* x
                                  int32_t act, void* stream) {
     const bool f8 = dtype == YMK_E4M3;
     if ((dtype != YMK_F32 && dtype != YMK_H16 && !f8) || (out_dtype != dtype && !(f8 && (out_dtype == YMK_F32 || out_dtype == YMK_H16))) ||
-        ex_bad_sizes(rows, E, Cin, Cout) || act < YMK_ACT_NONE || act > YMK_ACT_GELU || !offsets || (f8 && (!x_scale || !w_scale)) || (!f8 && (x_scale || w_scale)))
+        ex_bad_sizes(rows, E, Cin, Cout) || act < YMK_ACT_NONE || act > YMK_ACT_GELU || !offsets)
         return YMK_E_BADARG;
     const int es = f8 ? 1 : dtype == YMK_F32 ? 4 : 2, eo = out_dtype == YMK_F32 ? 4 : 2;
     if (rows == 0) return YMK_OK;
+    if ((f8 && (!x_scale || !w_scale)) || (!f8 && (x_scale || w_scale))) return YMK_E_BADARG;
     if (Cin * es % 16 || Cout % (f8 ? 8 : 16 / es) || ex_bad16(x) || ex_bad16(w) || ex_bad16(y) || ex_bad_ld(ldx, Cin, es) || ex_bad_ld(Cin, Cin, es) || ex_bad_ld(ldy, Cout, eo))
         return YMK_E_BADARG;
     const ExArgs a{static_cast<const char*>(w), static_cast<const char*>(x), static_cast<char*>(y), bias, w_scale, x_scale, offsets, nullptr,

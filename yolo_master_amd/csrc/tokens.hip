@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void token_dispatch_kernel(MoveArgs a) {
         const U v = *reinterpret_cast<const Any*>(a.x + t * a.ldx + at);
         for (int k = 0; k < a.top_k; ++k) {
             const int64_t r = a.rows[t * a.top_k + k];
-            if (r < 0) continue;
+            if ((uint64_t)r >= (uint64_t)(a.tokens * a.top_k)) continue;   // none, or no row of this plan
             *reinterpret_cast<Any*>(a.xs + r * a.ldxs + at) = v;
             if (a.scale && j == 0) a.xs_scale[r] = a.scale[t];
         }
@@ -238,6 +238,7 @@ __global__ __launch_bounds__(256) void token_combine_kernel(CombineArgs a) {
 #pragma unroll
             for (int k = 0; k < KU; ++k) {
                 r[k] = k0 + k < a.top_k ? a.row[t * a.top_k + k0 + k] : -1;
+                if (r[k] >= a.tokens * a.top_k) r[k] = -1;
                 w[k] = a.w && k0 + k < a.top_k ? a.w[t * a.top_k + k0 + k] : 1.0f;
             }
 #pragma unroll
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(256) void token_combine_backward_kernel(CombineBwdA
         for (int k = 0; k < a.top_k; ++k) {
             const int64_t r = a.row[t * a.top_k + k];
             float dot = 0.f;
-            if (r >= 0) {
+            if ((uint64_t)r < (uint64_t)(a.tokens * a.top_k)) {
                 const float w = a.w[t * a.top_k + k];
                 for (int j = lane; j < a.units; j += a.group) {
                     const int c = min(j * V, a.C - V), again = j * V - c;
