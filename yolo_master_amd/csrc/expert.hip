@@ -232,7 +232,8 @@ __device__ __forceinline__ bool ex_find(const ExArgs& a, ExTile& t) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e = c * 64 + lane;
-        first[c] = last[c] = 0;
+        first[c] = last[c] = incl[c] = 0;
+        if (c * 64 >= a.E) continue;   // for the whole wave
         if (e < a.E) {
             first[c] = min(max(a.offsets[e], 0), a.rows);
             last[c] = min(max(a.offsets[e + 1], first[c]), a.rows);
@@ -501,6 +502,15 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ExArgs a) {
     const char* wp[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) wp[i] = a.n + t.e * a.n_expert + (int64_t)min(t.n0 + i * 16 + r, a.N - 1) * a.n_ld;
+    // the epilogue's two channels of a row a thread; what it needs is fetched here
+    const int row = min(t.m0 + ((int)threadIdx.x >> 4), t.mend - 1), c = t.n0 + ((int)threadIdx.x & 15) * 2, ca = min(c, a.N - 2);   // N is even
+    const float ms = a.m_scale ? a.m_scale[row] : 1.f;
+    float scale[2], bias[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        scale[e] = a.n_scale ? ms * a.n_scale[(int64_t)t.e * a.N + ca + e] : 1.f;
+        bias[e] = a.bias ? a.bias[(int64_t)t.e * a.N + ca + e] : 0.f;
+    }
     const int bytes = a.K * ES, full = bytes >> 7;   // whole pieces of K; the rest is less than one
     f32x4 acc[NB];
 #pragma unroll
@@ -551,23 +561,19 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ExArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) part[wave][r][i * 16 + (lane >> 4) * 4 + q] = acc[i][q];
     __syncthreads();
-    const int row = t.m0 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 2;   // two channels of a row a thread
-    if (row >= t.mend || t.n0 + c >= a.N) return;                            // N is even
-    const float ms = a.m_scale ? a.m_scale[row] : 1.f;
+    if (t.m0 + ((int)threadIdx.x >> 4) >= t.mend || c >= a.N) return;
     float v[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const float(*p)[16][EX_FEW_N + 1] = part;
-        const int q = threadIdx.x >> 4;
-        v[e] = (p[0][q][c + e] + p[1][q][c + e]) + (p[2][q][c + e] + p[3][q][c + e]);
-        const int64_t at = (int64_t)t.e * a.N + t.n0 + c + e;
-        if (a.n_scale) v[e] *= ms * a.n_scale[at];
-        if (a.bias) v[e] += a.bias[at];
+        const int q = threadIdx.x >> 4, k = c - t.n0 + e;
+        v[e] = (p[0][q][k] + p[1][q][k]) + (p[2][q][k] + p[3][q][k]);
+        v[e] = std::is_same<T, E4m3>::value ? fmaf(v[e], scale[e], bias[e]) : v[e] + bias[e];
         if (a.act == YMK_ACT_SILU) v[e] = ex_act<YMK_ACT_SILU, sizeof(TO) == 2>(v[e]);
         else if (a.act == YMK_ACT_GELU) v[e] = ex_act<YMK_ACT_GELU, sizeof(TO) == 2>(v[e]);
         else if (a.act == YMK_ACT_SIGMOID) v[e] = ex_act<YMK_ACT_SIGMOID, sizeof(TO) == 2>(v[e]);
     }
-    TO* out = reinterpret_cast<TO*>(a.out) + (int64_t)row * a.out_ld + t.n0 + c;
+    TO* out = reinterpret_cast<TO*>(a.out) + (int64_t)row * a.out_ld + c;
     if constexpr (sizeof(TO) == 4) *reinterpret_cast<f32x2*>(out) = f32x2{v[0], v[1]};
     else *reinterpret_cast<uint32_t*>(out) = pack_h16x2(v[0], v[1]);
 }
