@@ -77,6 +77,11 @@ def test_plans_of_ones_own(ops):
     tc.check_plans_of_ones_own(ops)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_views(ops, dtype):
+    tc.check_views(ops, dtype)
+
+
 def test_dispatch_8bit(ops):
     tc.check_dispatch_8bit(ops)
 

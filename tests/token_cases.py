@@ -414,3 +414,29 @@ def check_plans_of_ones_own(ops, dev="cpu"):
     dys, dw = ops.token_combine_backward(x, ys, plan, w)
     close(dw, (part * x.cpu().double()[:, None]).sum(-1), torch.full((T, K), 1e-4), "dw")
     close(dys.cpu()[at], (w.cpu()[..., None] * x.cpu()[:, None])[good].double(), torch.full((len(at), C), 1e-6), "dys")
+
+
+def check_views(ops, dtype, dev="cpu"):
+    """Views that begin at any element, of one row, of three dims, and with rows far apart: the same bits as their dense copies."""
+    g = gen(21)
+    buf = torch.randn(9, 3, 70, generator=g).to(dtype).to(dev)
+    w = torch.rand(41, generator=g).to(dev)
+    for v in (buf[:, 1, 1:42], buf[:, :, 3:44], buf[2:3, 2, 5:46], buf[::2, 0, 7:48], buf[0, :, 29:]):
+        c = v.contiguous()
+        y, h, rstd = ops.rms_norm(v, w, residual=v)
+        y2, h2, rstd2 = ops.rms_norm(c, w, residual=c)
+        assert y.shape == v.shape and rstd.shape == v.shape[:-1] and torch.equal(y, y2) and torch.equal(h, h2) and torch.equal(rstd, rstd2)
+        q, s, _ = ops.rms_norm_quant(v, w)
+        q2, s2, _ = ops.rms_norm_quant(c, w)
+        assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s, s2)
+        dx, dw = ops.rms_norm_backward(v, h, w, rstd, dres=v)
+        dx2, dw2 = ops.rms_norm_backward(c, h2, w, rstd2, dres=c)
+        assert torch.equal(dx, dx2) and torch.equal(dw, dw2)
+        M = c.numel() // 41
+        plan = ops.token_sort((torch.arange(M)[:, None] % 3).to(torch.int32).to(dev), 3)
+        xs = ops.token_dispatch(v, plan)
+        assert torch.equal(xs, c.reshape(M, 41)[plan.src.long()])
+        assert torch.equal(ops.token_dispatch_backward(v, plan), c.reshape(M, 41)[plan.row[:, 0].long()])
+        gate = torch.ones(M, 1, device=dev)
+        a, b = ops.token_combine_backward(v, v, plan, gate), ops.token_combine_backward(c, c, plan, gate)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
