@@ -130,7 +130,7 @@ def check_norm_differences(ops, dev="cpu"):
 # ---------------------------------------------------------------------------------------------------------------- tokens
 # tokens, top_k, experts, share without an expert, int64 indexes
 SORTS = [(0, 2, 4, 0.0, False), (1, 1, 1, 0.0, False), (1, 2, 8, 0.0, True), (5, 3, 7, 0.4, False), (300, 2, 16, 0.0, False), (257, 16, 255, 0.1, True), (64, 1, 256, 1.0, False),
-         (4096, 2, 3, 0.0, False), (4097, 2, 5, 0.3, True), (9001, 1, 64, 0.05, False), (5000, 3, 256, 0.5, False), (8200, 1, 1, 0.5, False)]
+         (2048, 2, 5, 0.2, True), (1366, 3, 7, 0.0, False), (4096, 2, 3, 0.0, False), (4097, 2, 5, 0.3, True), (9001, 1, 64, 0.05, False), (5000, 3, 256, 0.5, False), (8200, 1, 1, 0.5, False)]
 
 
 def make_idx(g, T, K, E, dropped, wide):

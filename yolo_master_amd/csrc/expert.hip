@@ -14,7 +14,7 @@
 //
 // Measured (MI355X; a large library product reaches 1440 TFLOP/s in bf16, 2710 in e4m3, 154 in fp32, a large copy 5.0-5.4 TB/s): 32768 rows over 8 experts,
 // 1024 -> 4096 in bf16: y 291 us (945 TFLOP/s), dx 308, dW and db 283; 4096 -> 4096: 924 us (1190); 65532 rows over 32 experts, 2048 -> 4096 in e4m3 with
-// SiLU 614 us (1790).  What bounds it: the transfers (the loop without matrix instructions takes 0.85 of the whole, without transfers 0.8) and, where K is
+// SiLU 614 us (1790); other cards up to 6 % more.  What bounds it: the transfers (the loop without matrix instructions takes 0.85 of the whole, without transfers 0.8) and, where K is
 // short, the results' turn and the activation, which the one workgroup of a CU does not overlap with anything.  Workgroups that take tile after tile
 // and bring the next one's first step under the results of the last gained nothing (292 against 293 us, e4m3 778 against 568).
 //

@@ -2,9 +2,9 @@
 //
 // Memory-bound: a row is read once, kept in registers between the statistic and the output, and written once.  A row belongs to a group of
 // 2^n lanes (8..64 of one wave, or a whole workgroup of 128..1024): a lane holds up to NV vectors of V elements, vector i of lane l at column
-// (l + i * group) * V, so every load and store of a group is contiguous; V is 16 bytes (csrc/rows.h).  Groups of one wave need no LDS and no barrier, so they take every width that fits their registers once there are rows enough;
-// wide rows, and few rows, are spread over a workgroup.
-// Measured: residual sum, norm and e4m3 output of 25600 x 2048 bf16 70 us (5.3 TB/s); of 4 x 4096 4.2 us; 102400 x 256 bf16 forward 36 us (5.8 TB/s), gradients
+// (l + i * group) * V, so every load and store of a group is contiguous; V is 16 bytes (csrc/rows.h).  Groups of one wave
+// need no LDS and no barrier, so they take every width that fits their registers; wider rows are spread over a workgroup.
+// Measured: residual sum, norm and e4m3 output of 25600 x 2048 bf16 70 us (5.3 TB/s); of 4 x 4096 4.4 us; 102400 x 256 bf16 forward 36 us (5.8 TB/s), gradients
 // 37 + 5 us for dweight; 2041 x 1021 fp32 7.8 and 13 us (4.3 TB/s).
 #include "ymk_common.h"
 #include "rows.h"
@@ -303,8 +303,8 @@ __global__ __launch_bounds__(1024) void rms_norm_dweight_kernel(const float* par
 inline bool rn_al(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 inline bool rn_bad(const void* p, int32_t ld, int32_t C, int es) { return !p || ld < C || !rn_al(p, es); }
 
-// How a row of `vecs` vectors is spread: the group and the vectors a lane holds.  One wave holds up to 4 vectors a lane; with fewer rows than
-// the chip has waves a row is spread wider instead, down to one vector a lane (up to 1024 lanes), which shortens a single row's time.
+// How a row of `vecs` vectors is spread: the group and the vectors a lane holds.  (Few rows spread wider, down to one vector a lane, measured the same: 4
+// rows of 4096 7.3-7.6 us a call either way, 600 rows 7.2-7.3.)
 struct RnPlan {
     int group, nv, threads;
     unsigned grid;
@@ -312,10 +312,9 @@ struct RnPlan {
 // max_nv / wide_nv: vectors a lane may hold in workgroups of up to 256 lanes and in wider ones.
 inline RnPlan rn_plan(int64_t rows, int32_t vecs, int max_nv, int wide_nv, int64_t max_waves, int64_t max_groups) {
     RnPlan p;
-    const bool few = rows <= 512;
     p.group = 8;
-    while (p.group < 64 && p.group * (few ? 1 : 2) < vecs) p.group *= 2;
-    while (p.group < 1024 && p.group * (few ? 1 : p.group < 256 ? max_nv : wide_nv) < vecs) p.group *= 2;
+    while (p.group < 64 && p.group * 2 < vecs) p.group *= 2;
+    while (p.group < 1024 && p.group * (p.group < 256 ? max_nv : wide_nv) < vecs) p.group *= 2;
     p.nv = 1;
     while (p.group * p.nv < vecs) p.nv *= 2;
     p.threads = p.group > 64 ? p.group : 256;   // a group wider than a wave is a workgroup of its own
