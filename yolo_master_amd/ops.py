@@ -1364,7 +1364,7 @@ def rms_norm_backward(dy, h, weight, rstd, dres=None, need_dweight: bool = True)
 
 class TokenPlan(NamedTuple):
     """Where every (token, choice) pair goes: rows offsets[e] .. offsets[e + 1] are expert e's; src[row] = token * top_k + choice, -1 behind the last
-    row; row[token][choice] = its row, -1 for a pair without an expert.  All int32 on the device; the host never learns the counts."""
+    row; row[token][choice] = its row, -1 for a pair without an expert.  All dense int32 on the device; the host never learns the counts."""
 
     offsets: torch.Tensor
     src: torch.Tensor
@@ -1397,7 +1397,10 @@ def token_sort(idx, experts: int) -> TokenPlan:
 
 def _planned(what, plan, t, rows=None):
     """(tokens, top_k) of the plan; t has a row for every token, or (rows) for every pair."""
-    T, K = plan.row.shape
+    row = plan.row
+    if row.dtype is not torch.int32 or row.dim() != 2 or not row.is_contiguous():   # the kernels read it as dense int32
+        raise ValueError(f"{what}: plan.row is a contiguous int32 [tokens, top_k] tensor, got {row.dtype} {list(row.shape)} of strides {list(row.stride())}")
+    T, K = row.shape
     M, Cc, ld = _rows(t, what)
     if M != (T * K if rows else T) or Cc < 1:
         raise ValueError(f"{what}: {M} rows for a plan of {T} tokens by {K}")
