@@ -72,8 +72,9 @@ int ymk_token_combine_backward(int32_t dtype, const void* dy, int32_t lddy, cons
  *     y[r] = act(x[r] W[e]^T + bias[e]),   W dense [E][Cout][Cin] of x's type, bias fp32 [E][Cout] or NULL, act YMK_ACT_*.
  * dtype YMK_F32 | YMK_H16, out_dtype the same; or YMK_E4M3 (x and W in 8 bits, W[e][o] standing for W * w_scale[e][o], x[r] for
  * x * x_scale[r], both scales fp32 and required) with out_dtype YMK_F32 | YMK_H16.  Products are added in 32 bits and the sum (scaled,
- * with bias and activation) is rounded once; of 8-bit products the matrix instruction adds 16 at a time at the largest one's exponent, 13
- * bits deep, and those sums in 32 bits.  rows < 2^26.  offsets: device int32 [E + 1], ascending, within [0, rows] (values outside are clamped:
+ * with bias and activation) is rounded once.  One exception: 8-bit products with a 16-bit output and 32 rows an expert or more, where the matrix
+ * instruction adds 16 products at a time at the largest one's exponent, 13 bits deep, and those sums in 32 bits (1.5e-5 rms of the sum, under a
+ * tenth of the output's rounding).  rows < 2^26.  offsets: device int32 [E + 1], ascending, within [0, rows] (values outside are clamped:
  * no access leaves the tensors); rows outside every expert are left as they were.  Cin and Cout in multiples of 16 bytes of their
  * elements (4 fp32, 8 16-bit, 16 8-bit; Cout of 8 for YMK_E4M3), all pointers and row strides 16-byte aligned, strides below 2^23 bytes. */
 int ymk_expert_linear(int32_t dtype, int32_t out_dtype, const void* x, int32_t ldx, const float* x_scale, const void* w, const float* w_scale,

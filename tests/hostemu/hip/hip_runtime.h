@@ -343,6 +343,12 @@ static inline int __builtin_amdgcn_cvt_pk_fp8_f32(float x, float y, int old, boo
     const unsigned v = hostemu::to_e4m3(x) | (hostemu::to_e4m3(y) << 8);
     return (int)(high ? ((unsigned)old & 0xffffu) | (v << 16) : ((unsigned)old & 0xffff0000u) | v);
 }
+// two e4m3 codes of a word (its lower or upper half) times scale in bfloat16
+typedef __bf16 hostemu_bf16x2 __attribute__((ext_vector_type(2)));
+static inline hostemu_bf16x2 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(unsigned codes, float scale, bool high) {
+    const unsigned v = high ? codes >> 16 : codes;
+    return hostemu_bf16x2{(__bf16)(hostemu::from_e4m3(v & 255u) * scale), (__bf16)(hostemu::from_e4m3((v >> 8) & 255u) * scale)};
+}
 // ds_read_b64_tr_b16: the 16 lanes of a group read four rows of 16 16-bit elements, lane i the elements 4 (i % 4) .. + 3 of row i / 4 at its own
 // address, and lane i receives column i of them
 static inline hostemu_u32x2 hostemu_ds_read_tr16_b64(const char* p) {

@@ -1,0 +1,16 @@
+"""What tests/test_hostemu_token_edges.py checks of the token operators' kernels, on the GPU, where the matrix instructions' own sums show."""
+import pytest
+import torch
+
+from tests import token_cases as tc
+from tests.test_gpu_tokens import DEV, ops  # noqa: F401  (fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("case", tc.DEEP_FEW + tc.DEEP_MANY)
+def test_sums_of_8bit_products(ops, case):
+    tc.check_product_deep_sums(ops, case, torch.float32, DEV)
+    if case in tc.DEEP_FEW:
+        for dtype in (torch.bfloat16, torch.float16):
+            tc.check_product_deep_sums(ops, case, dtype, DEV)

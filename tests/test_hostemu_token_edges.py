@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests import token_cases as tc
-from tests.test_hostemu_tokens import DTYPES, libs, ops  # noqa: F401  (fixtures)
+from tests.test_hostemu_tokens import libs, ops  # noqa: F401  (fixtures)
 
 
 def test_a_plan_is_dense_int32(ops):
@@ -24,3 +24,11 @@ def test_a_plan_is_dense_int32(ops):
             with pytest.raises(ValueError, match="plan"):
                 call()
                 pytest.fail(f"{what} row was taken")
+
+
+@pytest.mark.parametrize("case", tc.DEEP_FEW + tc.DEEP_MANY)
+def test_sums_of_8bit_products(ops, case):
+    tc.check_product_deep_sums(ops, case, torch.float32)
+    if case in tc.DEEP_FEW:
+        for dtype in (torch.bfloat16, torch.float16):
+            tc.check_product_deep_sums(ops, case, dtype)

@@ -440,3 +440,30 @@ def check_views(ops, dtype, dev="cpu"):
         gate = torch.ones(M, 1, device=dev)
         a, b = ops.token_combine_backward(v, v, plan, gate), ops.token_combine_backward(c, c, plan, gate)
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# rows per expert, rows behind them, Cin, Cout: few rows (under 32 an expert, where 16-bit outputs come from 32-bit sums too), and many
+DEEP_FEW = [([1], 0, 16, 8), ([3, 0, 5, 1], 2, 1024, 48), ([2, 2, 0, 7], 0, 336, 136), ([16], 1, 1008, 40), ([9, 0, 70, 20], 0, 272, 72)]
+DEEP_MANY = [([130, 0, 1, 37], 3, 80, 144), ([64, 20], 0, 1024, 264), ([400, 301], 1, 496, 520)]
+
+
+def check_product_deep_sums(ops, case, out_dtype, dev="cpu"):
+    """8-bit products of -2^14 .. 2^14, whole numbers whose sums stay below 2^24: a sum held in 32 bits is exact in any order, and the output is that sum
+    rounded once (scales are powers of two).  Products that cancel leave the small ones, which an addition at fewer bits loses."""
+    counts, behind, Cin, Cout = case
+    g = gen(Cin * 5 + Cout)
+    E, rows = len(counts), sum(counts) + behind
+    whole = torch.arange(1, 129).float()
+    whole = whole[whole.to(torch.float8_e4m3fn).float() == whole]
+    pick = lambda *s: (whole[torch.randint(0, len(whole), s, generator=g)] * (2.0 * torch.randint(0, 2, s, generator=g) - 1))   # noqa: E731
+    x, w = pick(rows, Cin), pick(E, Cout, Cin)
+    x[:, 1:8:2], w[..., 1:8:2] = x[:, :8:2], -w[..., :8:2]   # neighbours cancel
+    x, w = x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn)
+    assert float((x.double().abs().max() * w.double().abs().max()) * Cin) <= 2.0**24
+    xs, ws = 2.0 ** torch.randint(-12, -9, (rows,), generator=g).float(), 2.0 ** torch.randint(-6, 0, (E, Cout), generator=g).float()
+    off = make_offsets(counts)
+    y = ops.expert_linear(x.to(dev), w.to(dev), off.to(dev), x_scale=xs.to(dev), w_scale=ws.to(dev), out_dtype=out_dtype).cpu()
+    for e, n in enumerate(counts):
+        s = slice(int(off[e]), int(off[e]) + n)
+        want = (x[s].double() @ w[e].double().t()) * xs[s].double()[:, None] * ws[e].double()
+        assert torch.equal(y[s], want.to(out_dtype)), (e, float((y[s].double() - want).abs().max()))
