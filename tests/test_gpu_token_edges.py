@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from tests import token_cases as tc
-from tests.test_gpu_tokens import DEV, ops  # noqa: F401  (fixture)
+from tests.test_gpu_tokens import DEV, DTYPES, ops  # noqa: F401  (fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -14,3 +14,8 @@ def test_sums_of_8bit_products(ops, case):
     if case in tc.DEEP_FEW:
         for dtype in (torch.bfloat16, torch.float16):
             tc.check_product_deep_sums(ops, case, dtype, DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_empty_batches(ops, dtype):
+    tc.check_empty_batches(ops, dtype, DEV)

@@ -32,3 +32,8 @@ def test_sums_of_8bit_products(ops, case):
     if case in tc.DEEP_FEW:
         for dtype in (torch.bfloat16, torch.float16):
             tc.check_product_deep_sums(ops, case, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_empty_batches(ops, dtype):
+    tc.check_empty_batches(ops, dtype)

@@ -467,3 +467,26 @@ def check_product_deep_sums(ops, case, out_dtype, dev="cpu"):
         s = slice(int(off[e]), int(off[e]) + n)
         want = (x[s].double() @ w[e].double().t()) * xs[s].double()[:, None] * ws[e].double()
         assert torch.equal(y[s], want.to(out_dtype)), (e, float((y[s].double() - want).abs().max()))
+
+
+def check_empty_batches(ops, dtype, dev="cpu"):
+    """No rows, in batches of any rank: outputs of the same rank without rows, zero sums over none of them."""
+    C, E, K = 16, 3, 2
+    w = torch.ones(C, device=dev)
+    wt = torch.ones(E, 8, C, dtype=dtype, device=dev)
+    plan = ops.token_sort(torch.zeros(0, K, dtype=torch.int32, device=dev), E)
+    gate = torch.zeros(0, K, device=dev)
+    for shape in ((0, C), (2, 0, C), (0, 2, C), (3, 0, 5, C), (2, 3, 0, C), (1, 0, 1, C)):
+        for x in (torch.zeros(shape, dtype=dtype, device=dev), torch.zeros(*shape[:-1], 2 * C, dtype=dtype, device=dev)[..., :C]):
+            y, h, rstd = ops.rms_norm(x, w, residual=x)
+            assert y.shape == h.shape == shape and rstd.shape == shape[:-1]
+            q, scale, _ = ops.rms_norm_quant(x, w, residual=x, residual_out=h)
+            assert q.shape == shape and scale.shape == shape[:-1]
+            dx, dw = ops.rms_norm_backward(x, h, w, rstd, dres=x)
+            assert dx.shape == shape and torch.equal(dw, torch.zeros_like(w))
+            assert ops.token_dispatch(x, plan).shape == (0, C) and ops.token_dispatch_backward(x, plan).shape == (0, C)
+            assert ops.token_combine(x, plan, gate).shape == (0, C) and ops.token_combine_backward(x, x, plan, gate)[0].shape == (0, C)
+            off = torch.zeros(E + 1, dtype=torch.int32, device=dev)
+            assert ops.expert_linear(x, wt, off).shape == (0, 8)
+            dx, dw, db = ops.expert_linear_backward(torch.zeros(0, 8, dtype=dtype, device=dev), x, wt, off)
+            assert dx.shape == (0, C) and torch.equal(dw, torch.zeros_like(wt)) and torch.equal(db, torch.zeros(E, 8, device=dev))

@@ -1220,6 +1220,8 @@ def _rows(t: torch.Tensor, what: str):
         ld, dense = strides
     elif len(shape) > 2:
         Cc, M, ld, dense = shape[-1], 1, 0, strides[-1]
+        if 0 in shape[:-1]:   # no rows, whatever the strides
+            return 0, Cc, Cc
         for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
             if n == 1:
                 continue
