@@ -37,3 +37,32 @@ def test_sums_of_8bit_products(ops, case):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_empty_batches(ops, dtype):
     tc.check_empty_batches(ops, dtype)
+
+
+def test_strides_that_do_not_fit_are_refused(ops):
+    """Row strides and widths go to the kernels as 32-bit numbers of elements (dispatch: 64-bit bytes): one of 2^32 + 16 must not arrive as 16."""
+    far = torch.empty(2**32 + 64, dtype=torch.bfloat16)   # never touched but for its ends
+    n, gate = 16, torch.ones(2, 1)
+    x = far.as_strided((2, n), (2**32 + 16, 1))
+    x[0], x[1] = 1, 2
+    near, w = torch.ones(2, n, dtype=torch.bfloat16), torch.ones(n)
+    plan = ops.token_sort(torch.tensor([[1], [0]], dtype=torch.int32), 2)
+    off = torch.tensor([0, 2], dtype=torch.int32)
+    wt = torch.ones(1, n, n, dtype=torch.bfloat16)
+    for bad in (lambda: ops.rms_norm(x, w), lambda: ops.rms_norm(near, w, residual=x), lambda: ops.rms_norm(near, w, residual=near, residual_out=x), lambda: ops.rms_norm_quant(x, w),
+                lambda: ops.rms_norm_backward(x, near, w, torch.ones(2)), lambda: ops.rms_norm_backward(near, x, w, torch.ones(2)),
+                lambda: ops.rms_norm_backward(near, near, w, torch.ones(2), dres=x), lambda: ops.token_combine(x, plan, gate), lambda: ops.token_dispatch_backward(x, plan),
+                lambda: ops.token_combine_backward(x, near, plan, gate), lambda: ops.token_combine_backward(near, x, plan, gate), lambda: ops.expert_linear(x, wt, off),
+                lambda: ops.expert_linear_backward(x, near, wt, off), lambda: ops.expert_linear_backward(near, x, wt, off)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            bad()
+    wide = far[:2**32 + 16].view(1, -1)
+    one = ops.token_sort(torch.zeros(1, 1, dtype=torch.int32), 1)
+    for bad in (lambda: ops.token_combine(wide, one, gate[:1]), lambda: ops.token_combine_backward(wide, wide, one, gate[:1]), lambda: ops.token_dispatch_backward(wide, one)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            bad()
+    assert torch.equal(ops.token_dispatch(x, plan), torch.tensor([[2.0], [1.0]]).expand(2, n).bfloat16())
+    m = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device="meta")   # noqa: E731
+    for bad in (lambda: ops.expert_linear(m(2, 8), m(1, 2**32 + 8, 8), off), lambda: ops.expert_linear_backward(m(2, 2**32 + 8), m(2, 8), m(1, 2**32 + 8, 8), off)):
+        with pytest.raises(ValueError, match="2\\^23"):
+            bad()

@@ -1209,10 +1209,10 @@ def _lib_for(dtype):
     return _lib._lib or _lib.load()
 
 
-def _rows(t: torch.Tensor, what: str):
-    """(rows, C, ld) of a row view."""
+def _rows(t: torch.Tensor, what: str, most: int = 2**31 - 1):
+    """(rows, C, ld) of a row view; C and ld fit the int32 that the C functions take (or most)."""
     shape = t.shape
-    if len(shape) == 2 and t.is_contiguous() and shape[1]:
+    if len(shape) == 2 and t.is_contiguous() and 0 < shape[1] <= most:
         return shape[0], shape[1], shape[1]
     strides = t.stride()
     if len(shape) == 2:
@@ -1234,6 +1234,8 @@ def _rows(t: torch.Tensor, what: str):
         raise ValueError(f"{what}: expected [..., C], got {tuple(shape)}")
     if dense != 1 and Cc > 1:
         raise ValueError(f"{what}: the last dim must be dense")
+    if Cc > most or M > 1 and ld > most:
+        raise ValueError(f"{what}: rows of {Cc} elements at a stride of {ld}, 2^31 or more")
     if M <= 1:
         return M, Cc, Cc
     if ld < Cc:
@@ -1397,13 +1399,13 @@ def token_sort(idx, experts: int) -> TokenPlan:
     return TokenPlan(offsets, src, row, experts)
 
 
-def _planned(what, plan, t, rows=None):
+def _planned(what, plan, t, rows=None, **most):
     """(tokens, top_k) of the plan; t has a row for every token, or (rows) for every pair."""
     row = plan.row
     if row.dtype is not torch.int32 or row.dim() != 2 or not row.is_contiguous():   # the kernels read it as dense int32
         raise ValueError(f"{what}: plan.row is a contiguous int32 [tokens, top_k] tensor, got {row.dtype} {list(row.shape)} of strides {list(row.stride())}")
     T, K = row.shape
-    M, Cc, ld = _rows(t, what)
+    M, Cc, ld = _rows(t, what, **most)
     if M != (T * K if rows else T) or Cc < 1:
         raise ValueError(f"{what}: {M} rows for a plan of {T} tokens by {K}")
     return T, K, Cc, ld
@@ -1414,7 +1416,7 @@ def token_dispatch(x, plan: TokenPlan, scale=None):
     """xs[plan.row[t][k]] = x[t], any element type; with scale (fp32 [tokens], of an 8-bit x) -> (xs, xs_scale).  Rows behind the last expert's are
     not written."""
     stream = _here("token_dispatch", x, plan.row, scale)
-    T, K, Cc, ldx = _planned("token_dispatch", plan, x)
+    T, K, Cc, ldx = _planned("token_dispatch", plan, x, most=2**59)   # strides in bytes, int64
     es = x.element_size()
     xs = x.new_empty(T * K, Cc)
     xs_scale = None
@@ -1480,6 +1482,8 @@ def _expert_args(what, x, w, offsets):
     E, Cout, Cin = w.shape
     if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or not offsets.is_contiguous():
         raise ValueError(f"{what}: offsets is a contiguous int32 [{E + 1}] tensor")
+    if Cin >= 1 << 23 or Cout >= 1 << 23:   # rows of 2^23 bytes and more, refused below too; the C functions take int32
+        raise ValueError(f"{what}: {Cin} -> {Cout} channels (below 2^23)")
     if E > _lib.TOKEN_MAX_E:
         raise ValueError(f"{what}: {E} experts (at most {_lib.TOKEN_MAX_E})")
     return E, Cout, Cin
