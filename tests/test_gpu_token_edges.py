@@ -19,3 +19,8 @@ def test_sums_of_8bit_products(ops, case):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_empty_batches(ops, dtype):
     tc.check_empty_batches(ops, dtype, DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_residual_out_beside_an_input(ops, dtype):
+    tc.check_residual_out_beside(ops, dtype, DEV)

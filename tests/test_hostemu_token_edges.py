@@ -66,3 +66,16 @@ def test_strides_that_do_not_fit_are_refused(ops):
     for bad in (lambda: ops.expert_linear(m(2, 8), m(1, 2**32 + 8, 8), off), lambda: ops.expert_linear_backward(m(2, 2**32 + 8), m(2, 8), m(1, 2**32 + 8, 8), off)):
         with pytest.raises(ValueError, match="2\\^23"):
             bad()
+
+
+def test_residual_out_beside_an_input(ops):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        tc.check_residual_out_beside(ops, dtype)
+    buf, r, w = torch.zeros(6, 96), torch.zeros(4, 40), torch.ones(40)
+    for out in (buf[:4, 1:41], buf[:4, 39:79], buf[1:5, :40], buf.view(-1)[160:544].view(4, 96)[:, :40], buf.view(-1)[41:341].view(4, 75)[:, :40]):   # shifted, a row on, the end of the row before, other strides
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.rms_norm(buf[:4, :40], w, residual=r, residual_out=out)
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.rms_norm(r, w, residual=buf[:4, :40], residual_out=out)
+    for out in (buf[2:6, 56:], buf[1:5, 40:80]):   # other rows' columns 56 .. 95 and 40 .. 79: none of x's 0 .. 39
+        assert ops.rms_norm(buf[:4, :40], w, residual=r, residual_out=out)[1] is out

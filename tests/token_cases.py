@@ -490,3 +490,20 @@ def check_empty_batches(ops, dtype, dev="cpu"):
             assert ops.expert_linear(x, wt, off).shape == (0, 8)
             dx, dw, db = ops.expert_linear_backward(torch.zeros(0, 8, dtype=dtype, device=dev), x, wt, off)
             assert dx.shape == (0, C) and torch.equal(dw, torch.zeros_like(wt)) and torch.equal(db, torch.zeros(E, 8, device=dev))
+
+
+def check_residual_out_beside(ops, dtype, dev="cpu"):
+    """h written to the other part of the rows that x or the residual lies in: no element is shared, and nothing else of the buffer changes."""
+    g = gen(31)
+    w = torch.rand(40, generator=g).to(dev)
+    for T, width, at, to in ((5, 80, 0, 40), (5, 80, 40, 0), (7, 123, 3, 83), (1, 80, 0, 40), (6, 200, 100, 17)):
+        buf = torch.randn(T, width, generator=g).to(dtype).to(dev)
+        other = rows_of(g, T, 40, dtype, 0, dev)
+        for swap in (False, True):
+            b = buf.clone()
+            x, r = (other, b[:, at:at + 40]) if swap else (b[:, at:at + 40], other)
+            y, h, rstd = ops.rms_norm(x.clone(), w, residual=r.clone())
+            y2, h2, rstd2 = ops.rms_norm(x, w, residual=r, residual_out=b[:, to:to + 40])
+            want = buf.clone()
+            want[:, to:to + 40] = h
+            assert torch.equal(y, y2) and torch.equal(h, h2) and torch.equal(rstd, rstd2) and torch.equal(b, want)

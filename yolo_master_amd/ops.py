@@ -1302,10 +1302,12 @@ def _norm_args(what, x, weight, residual, residual_out):
     if residual_out is None:
         return stream, M, Cc, ldx, ldr, _new(x, dt), Cc
     ldh = _like(residual_out, x, what, "residual_out")
-    for t, ld in ((x, ldx), (residual, ldr)):   # in place is fine, row by row; a shifted view is not
-        a, b = t.data_ptr(), residual_out.data_ptr()
-        span = ((M - 1) * max(ld, ldh) + Cc) * x.element_size()
-        if M and not (a == b and (ld == ldh or M == 1)) and abs(a - b) < span:
+    es = x.element_size()
+    for t, ld in ((x, ldx), (residual, ldr)):   # in place is fine, row by row, and so is another part of the same rows; a shifted view is not
+        apart = abs(t.data_ptr() - residual_out.data_ptr())
+        if M == 0 or apart >= ((M - 1) * max(ld, ldh) + Cc) * es or apart == 0 and (ld == ldh or M == 1):
+            continue
+        if ld != ldh or not Cc * es <= apart % (ld * es) <= (ld - Cc) * es:
             raise ValueError(f"{what}: residual_out overlaps an input without being it")
     return stream, M, Cc, ldx, ldr, residual_out, ldh
 
@@ -1313,7 +1315,8 @@ def _norm_args(what, x, weight, residual, residual_out):
 @_timed("rms_norm")
 def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
     """h = x + residual (rounded to x's dtype; h is x without a residual), y = h / sqrt(mean(h^2) + eps) * weight.  Returns (y, h, rstd); rstd
-    fp32, one a row, is what rms_norm_backward takes.  residual_out: where h goes (x or residual themselves, or a tensor apart from them)."""
+    fp32, one a row, is what rms_norm_backward takes.  residual_out: where h goes (x or residual themselves, or elements of
+    neither, also of the same rows)."""
     stream, M, Cc, ldx, ldr, h, ldh = _norm_args("rms_norm", x, weight, residual, residual_out)
     dt = x.dtype
     y, rstd = _new(x, dt), _new_stat(x, M, weight)
