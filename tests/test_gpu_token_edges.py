@@ -24,3 +24,11 @@ def test_empty_batches(ops, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_residual_out_beside_an_input(ops, dtype):
     tc.check_residual_out_beside(ops, dtype, DEV)
+
+
+@pytest.mark.parametrize("act", [None, "silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_activations_of_sums_that_are_not_finite(ops, act, rows):
+    for dtype in DTYPES:
+        tc.check_activations(ops, dtype, act, rows, dev=DEV)
+        tc.check_activations(ops, torch.float8_e4m3fn, act, rows, dtype, DEV)

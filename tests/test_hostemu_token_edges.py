@@ -79,3 +79,11 @@ def test_residual_out_beside_an_input(ops):
             ops.rms_norm(r, w, residual=buf[:4, :40], residual_out=out)
     for out in (buf[2:6, 56:], buf[1:5, 40:80]):   # other rows' columns 56 .. 95 and 40 .. 79: none of x's 0 .. 39
         assert ops.rms_norm(buf[:4, :40], w, residual=r, residual_out=out)[1] is out
+
+
+@pytest.mark.parametrize("act", [None, "silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_activations_of_sums_that_are_not_finite(ops, act, rows):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        tc.check_activations(ops, dtype, act, rows)
+        tc.check_activations(ops, torch.float8_e4m3fn, act, rows, dtype)

@@ -507,3 +507,28 @@ def check_residual_out_beside(ops, dtype, dev="cpu"):
             want = buf.clone()
             want[:, to:to + 40] = h
             assert torch.equal(y, y2) and torch.equal(h, h2) and torch.equal(rstd, rstd2) and torch.equal(b, want)
+
+
+def check_activations(ops, dtype, act, rows, out_dtype=None, dev="cpu"):
+    """act of sums that are not finite, huge, tiny, and in the tails: the bias alone makes them (x is zero).  Not-a-number and infinities come out where the
+    definition has them.  Finite values: short forms (16-bit outputs) round the exponent's argument, at most 89 here, to half of 2^-17, and their
+    reciprocal gives zero for results below 2^-118; exact ones (fp32) add 1 + erf to half of 2^-23 and multiply by v / 2."""
+    inf, nan = float("inf"), float("nan")
+    b = torch.cat([torch.tensor([inf, -inf, nan, 0.0, -0.0, 1e30, -1e30, 3e38, -3e38, 6e4, -6e4, 1e-30, -1e-30]), torch.linspace(-100, 100, 203)])
+    E, Cin, Cout = 1, 16, b.numel()
+    f8 = dtype == torch.float8_e4m3fn
+    x, w = torch.zeros(rows, Cin, dtype=dtype, device=dev), torch.ones(E, Cout, Cin).to(dtype).to(dev)
+    scales = {"x_scale": torch.ones(rows, device=dev), "w_scale": torch.ones(E, Cout, device=dev), "out_dtype": out_dtype} if f8 else {}
+    y = ops.expert_linear(x, w, make_offsets([rows]).to(dev), b[None].to(dev), act=act, **scales).cpu()
+    odt = out_dtype or dtype
+    v = b.double()
+    want = 0.5 * v * torch.special.erfc(-v * 0.5**0.5) if act == "gelu" else act64(v, act)   # 1 + erf would leave 2^-53 of the tail
+    stored = want.to(odt)
+    for r in range(rows):
+        assert torch.equal(torch.isnan(y[r]), torch.isnan(stored)), (r, b[torch.isnan(y[r]) != torch.isnan(stored)])
+        assert torch.equal(torch.isinf(y[r]), torch.isinf(stored)) and torch.equal(y[r][torch.isinf(stored)], stored[torch.isinf(stored)])
+        f = torch.isfinite(stored)
+        tol = want.abs() * (half(odt) + (2.0**-17 if half(odt) > U else 8 * U)) + TINY[odt] + (2.0**-118 if half(odt) > U else 0.0)
+        if half(odt) == U:
+            tol = tol + v.abs().clamp_max(1e30) * (2 * U) * (v < 0) + 2.0**-126
+        close(y[r][f], want[f], tol[f], f"{act} row {r}")

@@ -298,8 +298,9 @@ __device__ __forceinline__ bool ex_find(const ExArgs& a, ExTile& t) {
     return false;
 }
 
-// The activation of an fp32 output in the exact forms; of a 16-bit one in short forms of a few units of 2^-23 (the exact ones take about 50 instructions an
-// element, more than the products of a 2048-wide row).  GELU = x Phi(x) through erfc(z) = t exp(-z^2 + p(t)), t = 1 / (1 + z / 2): the Chebyshev fit
+// The activation of an fp32 output in the exact forms; of a 16-bit one in short forms (the exact ones take about 50 instructions an element, more
+// than the products of a 2048-wide row): a few units of 2^-23 around zero, up to 2^-17 where the exponential's argument is near its end (rounded at 2^-18
+// there), zero for results below 2^-118 (a reciprocal that is subnormal).  GELU = x Phi(x) through erfc(z) = t exp(-z^2 + p(t)), t = 1 / (1 + z / 2): the Chebyshev fit
 // of Press et al., Numerical Recipes (2nd ed., 6.2), relative error 1.2e-7 everywhere, so the negative tail keeps its digits.
 template <int ACT, bool SHORT>
 __device__ __forceinline__ float ex_act(float v) {
@@ -319,7 +320,7 @@ __device__ __forceinline__ float ex_act(float v) {
         p = fmaf(p, t, 1.00002368f);
         p = fmaf(p, t, -1.26551223f);
         const float half_erfc = 0.5f * t * __expf(fmaf(-z, z, p));
-        return v > 0.f ? v - v * half_erfc : v * half_erfc;
+        return v * (v > 0.f ? 1.0f - half_erfc : half_erfc);   // +infinity stays: v - v * 0 would be no number
     } else return v;
 }
 
