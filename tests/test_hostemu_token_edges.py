@@ -87,3 +87,14 @@ def test_activations_of_sums_that_are_not_finite(ops, act, rows):
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
         tc.check_activations(ops, dtype, act, rows)
         tc.check_activations(ops, torch.float8_e4m3fn, act, rows, dtype)
+
+
+def test_residual_out_right_behind_an_input(ops):
+    """Tensors apart from each other, with rows of different strides, at neighbouring addresses (as an allocator hands them out)."""
+    pool, w = torch.randn(2000), torch.ones(40)
+    dense, far = pool[:200].view(5, 40), pool[200:600].view(5, 80)[:, :40]
+    behind = pool[600:800].view(5, 40)   # from the end of the strided rows' last padding on
+    for x, out in ((dense, far), (far, behind), (behind, far), (far, dense)):
+        want = ops.rms_norm(x.clone(), w, residual=torch.ones(5, 40))
+        got = ops.rms_norm(x, w, residual=torch.ones(5, 40), residual_out=out)
+        assert torch.equal(got[0], want[0]) and torch.equal(out, want[1])

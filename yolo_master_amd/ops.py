@@ -1304,10 +1304,10 @@ def _norm_args(what, x, weight, residual, residual_out):
     ldh = _like(residual_out, x, what, "residual_out")
     es = x.element_size()
     for t, ld in ((x, ldx), (residual, ldr)):   # in place is fine, row by row, and so is another part of the same rows; a shifted view is not
-        apart = abs(t.data_ptr() - residual_out.data_ptr())
-        if M == 0 or apart >= ((M - 1) * max(ld, ldh) + Cc) * es or apart == 0 and (ld == ldh or M == 1):
-            continue
-        if ld != ldh or not Cc * es <= apart % (ld * es) <= (ld - Cc) * es:
+        apart = residual_out.data_ptr() - t.data_ptr()
+        if M == 0 or abs(apart) >= ((M - 1) * (ld if apart > 0 else ldh) + Cc) * es or apart == 0 and (ld == ldh or M == 1):
+            continue   # the lower one ends before the other begins, or it is the other
+        if ld != ldh or not Cc * es <= abs(apart) % (ld * es) <= (ld - Cc) * es:
             raise ValueError(f"{what}: residual_out overlaps an input without being it")
     return stream, M, Cc, ldx, ldr, residual_out, ldh
 
