@@ -52,14 +52,14 @@ size_t ymk_token_sort_workspace_bytes(int64_t tokens, int32_t top_k, int32_t E);
 int ymk_token_sort(const void* idx, int32_t idx_bytes, int64_t tokens, int32_t top_k, int32_t E, int32_t* offsets, int32_t* src,
                    int32_t* row, void* workspace, size_t workspace_bytes, void* stream);
 
-/* xs[row[t][k]] = x[t], byte for byte (any element type): row_bytes of a row, strides in bytes; with scale fp32 [tokens] (may be NULL)
+/* xs[row[t][k]] = x[t], byte for byte (any element type): row_bytes of a row (at most 2^24), strides in bytes; with scale fp32 [tokens] (may be NULL)
  * also xs_scale[row[t][k]] = scale[t].  Rows behind the last one are left as they were.  Here and below a row outside [0, tokens * top_k) is
  * no row. */
 int ymk_token_dispatch(const void* x, int64_t ldx_bytes, int64_t row_bytes, const float* scale, void* xs, int64_t ldxs_bytes,
                        float* xs_scale, const int32_t* row, int64_t tokens, int32_t top_k, void* stream);
 
 /* y[t] = sum over k of w[t][k] * ys[row[t][k]] in fp32, in the order of k, rounded once; pairs without a row add nothing (a token that
- * has none gets zeros).  w fp32 [tokens][top_k], NULL = ones: that is the gradient of ymk_token_dispatch. */
+ * has none gets zeros).  w fp32 [tokens][top_k], NULL = ones: that is the gradient of ymk_token_dispatch.  C <= 2^31 - 16, here and below. */
 int ymk_token_combine(int32_t dtype, const void* ys, int32_t ldys, const int32_t* row, const float* w, void* y, int32_t ldy, int64_t tokens,
                       int32_t top_k, int32_t C, void* stream);
 

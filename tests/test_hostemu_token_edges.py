@@ -98,3 +98,17 @@ def test_residual_out_right_behind_an_input(ops):
         want = ops.rms_norm(x.clone(), w, residual=torch.ones(5, 40))
         got = ops.rms_norm(x, w, residual=torch.ones(5, 40), residual_out=out)
         assert torch.equal(got[0], want[0]) and torch.equal(out, want[1])
+
+
+def test_rows_too_wide_for_the_kernels_counters(libs):
+    """Column numbers of the moves are 32-bit: a width whose round-up to whole vectors passes 2^31 is refused, not walked from a negative column."""
+    h = libs[False]
+    t = torch.full((64,), 5.0)
+    row = torch.zeros(1, dtype=torch.int32)
+    p, r = t.data_ptr(), row.data_ptr()
+    for dtype in (0, 1):
+        for wide in (2**31 - 15, 2**31 - 7, 2**31 - 1):
+            assert h.ymk_token_combine(dtype, p, wide, r, p, p, wide, 1, 1, wide, None) == -1
+            assert h.ymk_token_combine_backward(dtype, p, wide, p, wide, r, p, p, wide, p, 1, 1, wide, None) == -1
+    assert h.ymk_token_dispatch(p, 2**24 + 1, 2**24 + 1, None, p, 2**24 + 1, None, r, 1, 1, None) == -1
+    assert bool((t == 5).all())

@@ -12,6 +12,7 @@
 #else
 #define TK_MAX_BLOCKS YMK_MAX_BLOCKS
 #endif
+#define TK_MAX_C 0x7ffffff0   // widest row of the sums: the kernels count columns in 32 bits, a row rounded up to whole vectors included
 #define TK_SORT_BLOCKS 256    // most workgroups of the two-launch sort: each sums the histograms of those before it
 // Pairs that one workgroup sorts alone, in one launch: with one / two launches 7.6 / 10.5 us for 4096 pairs, 9.4 / 10.2 (16 experts) and 12.1 / 10.0 (128)
 // for 8192, 16.1 / 10.2 for 16384
@@ -360,7 +361,7 @@ extern "C" int ymk_token_dispatch(const void* x, int64_t ldx_bytes, int64_t row_
 
 extern "C" int ymk_token_combine(int32_t dtype, const void* ys, int32_t ldys, const int32_t* row, const float* w, void* y, int32_t ldy, int64_t tokens,
                                  int32_t top_k, int32_t C, void* stream) {
-    if ((dtype != YMK_F32 && dtype != YMK_H16) || tk_bad_plan(tokens, top_k) || C < 1 || ldys < C || ldy < C) return YMK_E_BADARG;
+    if ((dtype != YMK_F32 && dtype != YMK_H16) || tk_bad_plan(tokens, top_k) || C < 1 || C > TK_MAX_C || ldys < C || ldy < C) return YMK_E_BADARG;
     if (tokens == 0) return YMK_OK;
     const int es = dtype == YMK_F32 ? 4 : 2;
     if (!ys || !row || !y || !tk_al(ys, es) || !tk_al(y, es)) return YMK_E_BADARG;
@@ -372,7 +373,7 @@ extern "C" int ymk_token_combine(int32_t dtype, const void* ys, int32_t ldys, co
 
 extern "C" int ymk_token_combine_backward(int32_t dtype, const void* dy, int32_t lddy, const void* ys, int32_t ldys, const int32_t* row, const float* w,
                                           void* dys, int32_t lddys, float* dw, int64_t tokens, int32_t top_k, int32_t C, void* stream) {
-    if ((dtype != YMK_F32 && dtype != YMK_H16) || tk_bad_plan(tokens, top_k) || C < 1 || lddy < C || ldys < C || lddys < C) return YMK_E_BADARG;
+    if ((dtype != YMK_F32 && dtype != YMK_H16) || tk_bad_plan(tokens, top_k) || C < 1 || C > TK_MAX_C || lddy < C || ldys < C || lddys < C) return YMK_E_BADARG;
     if (tokens == 0) return YMK_OK;
     const int es = dtype == YMK_F32 ? 4 : 2;
     if (!dy || !ys || !row || !w || !dys || !dw || !tk_al(dy, es) || !tk_al(ys, es) || !tk_al(dys, es)) return YMK_E_BADARG;
