@@ -24,10 +24,12 @@ def test_the_two_hashes_hold_their_own_sources(monkeypatch, tmp_path):
     monkeypatch.setattr(build, "CSRC", tmp_path)
     assert (build.source_hash(), build.source_hash(tokens=True)) == before
     for f, detector, tokens in (("expert.hip", False, True), ("rows.h", False, True), ("dwconv.hip", True, False), ("glds.h", True, True)):
-        (tmp_path / f).write_bytes((tmp_path / f).read_bytes() + b"\n")
+        (tmp_path / f).write_text((tmp_path / f).read_text() + "\nint one_more;   // and a comment\n")
         now = build.source_hash(), build.source_hash(tokens=True)
         assert (now[0] != before[0], now[1] != before[1]) == (detector, tokens), f
         before = now
+        (tmp_path / f).write_text("// 12 us\n" + (tmp_path / f).read_text().replace("and a comment", "another") + "/* two\nlines */\n")
+        assert (build.source_hash(), build.source_hash(tokens=True)) == before   # comments are not the kernel
 
 
 def test_objects_of_other_flags_are_stale(monkeypatch, tmp_path):

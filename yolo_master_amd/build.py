@@ -52,15 +52,17 @@ def _flags(src: str, defs: list) -> list:
 
 def source_hash(tokens: bool = False) -> str:
     """sha256 (16 hex digits) over the detector's kernel sources (or the token operators'), their shared headers and the flags that each is compiled
-    with: committed rocprofv3 summaries carry it, so that a profile is only ever quoted for the kernels it was collected on (bench.py
+    with, comments aside (they quote what a profile measured): committed rocprofv3 summaries carry it, so that a profile is only ever quoted for the kernels it was collected on (bench.py
     `roofline.traffic`, `families[].sq`)."""
     import hashlib
+    import re
 
     h = hashlib.sha256()
     sources, headers = (TOKEN_SOURCES, ["ymk_common.h", "rows.h", "glds.h"]) if tokens else (set(SOURCES) - set(TOKEN_SOURCES), ["ymk_common.h", "igemm.h", "glds.h"])
     for f in sorted(sources) + headers:
         h.update(f.encode())
-        h.update((CSRC / f).read_bytes())
+        code = re.sub(r"//[^\n]*|/\*.*?\*/", "", (CSRC / f).read_text(), flags=re.S)
+        h.update("\n".join(line.rstrip() for line in code.splitlines() if line.strip()).encode())
         if f.endswith(".hip"):
             h.update(" ".join(_flags(f, [])).encode())
     return h.hexdigest()[:16]

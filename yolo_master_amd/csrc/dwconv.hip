@@ -7,8 +7,8 @@
 // already in flight into registers (coalesced 16-byte loads), so the HBM/L2 latency of a tile hides behind the
 // previous tile's arithmetic.  The LDS pixel stride is padded to 40 (bf16) / 80 (fp32) bytes so the x-strips of a
 // wave land on disjoint bank groups.  Each thread owns 4 channels x 10 consecutive output pixels of a row: per
-// filter row it streams 10+k-1 LDS vectors once and keeps the k taps in registers, accumulating with packed fp32
-// FMAs (v_pk_fma_f32 on two channel pairs).  The stencil has no contraction shared between channels, so MFMA does
+// filter row it streams 10+k-1 LDS vectors once and keeps the k taps in registers, accumulating in fp32, two
+// channel pairs at a time (a v_fma_f32 a channel: the build keeps packed fp32 instructions out).  The stencil has no contraction shared between channels, so MFMA does
 // not apply; the halo re-read is served by L2.
 //
 // Reference semantics: DWConv (ultralytics/nn/modules/conv.py:185-199), AAttn.pe
@@ -33,8 +33,8 @@
 //   3  PAIR-DOT (default since the dot2 form was measured): mode 2's planes with the two pixels of a 16-byte slot INTERLEAVED per channel — a
 //      32-bit word = (pixel 2j, pixel 2j + 1) of one channel — and the filter rows stored as tap pairs, so that the arithmetic is
 //      v_dot2_f32_bf16 (two multiply-adds per instruction straight from the 16-bit words) instead of widening shifts / masks +
-//      v_pk_fma_f32: (K + 1) / 2 dot2 per output and channel and filter row, no widening (K = 9: 200 VALU instructions per thread and
-//      row instead of 180 + 108).  Output pixel r even pairs its taps (0,1)(2,3)...; r odd pairs (-,0)(1,2)(3,4)... against the same words.
+//      FMAs: (K + 1) / 2 dot2 per output and channel and filter row, no widening (K = 9: 200 VALU instructions per thread and row
+//      instead of 360 + 108; 180 + 108 when the two were compared, by a build with packed fp32 FMAs).  Output pixel r even pairs its taps (0,1)(2,3)...; r odd pairs (-,0)(1,2)(3,4)... against the same words.
 #ifndef DW_LDS_MODE
 #define DW_LDS_MODE 3
 #endif
@@ -241,7 +241,7 @@ __device__ __forceinline__ void dw_run(const T* __restrict__ xb, int H, int W, i
         for (int ky = 0; ky < ((DW_ABLATE & 4) ? 1 : K); ++ky) {
             // ALL LDS reads of this filter row (K taps + DW_R + K - 1 pixels) are issued before the first use.  Left to itself the
             // compiler reads one or two operands at a time and waits for each (`ds_read2_b64; s_waitcnt lgkmcnt(0)`, 14 times per row at
-            // k = 9): one LDS round trip per pair of operands beside ~20 packed FMAs — what kept this kernel at 0.4 of the VALU rate
+            // k = 9): one LDS round trip per pair of operands beside ~40 FMAs — what kept this kernel at 0.4 of the VALU rate
             // with four waves per SIMD (found in the ISA of the round-4 one-kernel form's stencil, tools/micro/parked/esfused.hip.txt).  Same arithmetic, same order.
             typedef typename Raw4<T>::type raw_t;
             raw_t rw[K + 1], rd[DW_R + K - 1];
