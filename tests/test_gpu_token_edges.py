@@ -32,3 +32,8 @@ def test_activations_of_sums_that_are_not_finite(ops, act, rows):
     for dtype in DTYPES:
         tc.check_activations(ops, dtype, act, rows, dev=DEV)
         tc.check_activations(ops, torch.float8_e4m3fn, act, rows, dtype, DEV)
+
+
+@pytest.mark.parametrize("counts", [[2], [30, 9], [90, 70]])
+def test_scales_whose_product_is_subnormal(ops, counts):
+    tc.check_product_small_scales(ops, counts, DEV)

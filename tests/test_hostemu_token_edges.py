@@ -112,3 +112,8 @@ def test_rows_too_wide_for_the_kernels_counters(libs):
             assert h.ymk_token_combine_backward(dtype, p, wide, p, wide, r, p, p, wide, p, 1, 1, wide, None) == -1
     assert h.ymk_token_dispatch(p, 2**24 + 1, 2**24 + 1, None, p, 2**24 + 1, None, r, 1, 1, None) == -1
     assert bool((t == 5).all())
+
+
+@pytest.mark.parametrize("counts", [[2], [30, 9]])
+def test_scales_whose_product_is_subnormal(ops, counts):
+    tc.check_product_small_scales(ops, counts)

@@ -532,3 +532,15 @@ def check_activations(ops, dtype, act, rows, out_dtype=None, dev="cpu"):
         if half(odt) == U:
             tol = tol + v.abs().clamp_max(1e30) * (2 * U) * (v < 0) + 2.0**-126
         close(y[r][f], want[f], tol[f], f"{act} row {r}")
+
+
+def check_product_small_scales(ops, counts, dev="cpu"):
+    """Scales whose product is no normal number while the sum's is one: each is multiplied in for itself."""
+    Cin, Cout, E = 4096, 16, len(counts)
+    rows = sum(counts)
+    x, w = torch.full((rows, Cin), 448.0).to(torch.float8_e4m3fn), torch.full((E, Cout, Cin), 448.0).to(torch.float8_e4m3fn)
+    xs, ws = torch.full((rows,), 3e-23), torch.full((E, Cout), 3.1e-23)
+    want = 448.0**2 * Cin * float(xs[0]) * float(ws[0, 0])
+    for dtype in (torch.float32, torch.bfloat16):
+        y = ops.expert_linear(x.to(dev), w.to(dev), make_offsets(counts).to(dev), x_scale=xs.to(dev), w_scale=ws.to(dev), out_dtype=dtype)
+        close(y, torch.full((rows, Cout), want, dtype=torch.float64), torch.full((rows, Cout), want * (half(dtype) + (Cin + 8) * U)), "small scales")

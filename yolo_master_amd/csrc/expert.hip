@@ -538,7 +538,7 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ExArgs a) {
     float scale[2], bias[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-        scale[e] = a.n_scale ? ms * a.n_scale[(int64_t)t.e * a.N + ca + e] : 1.f;
+        scale[e] = a.n_scale ? a.n_scale[(int64_t)t.e * a.N + ca + e] : 1.f;
         bias[e] = a.bias ? a.bias[(int64_t)t.e * a.N + ca + e] : 0.f;
     }
     const int bytes = a.K * ES, full = bytes >> 7;   // whole pieces of K; the rest is less than one
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ExArgs a) {
         const float(*p)[16][EX_FEW_N + 1] = part;
         const int q = threadIdx.x >> 4, k = c - t.n0 + e;
         v[e] = (p[0][q][k] + p[1][q][k]) + (p[2][q][k] + p[3][q][k]);
-        v[e] = std::is_same<T, E4m3>::value ? fmaf(v[e], scale[e], bias[e]) : v[e] + bias[e];
+        v[e] = std::is_same<T, E4m3>::value ? fmaf(v[e] * ms, scale[e], bias[e]) : v[e] + bias[e];   // the scales' product may be subnormal
         if (a.act == YMK_ACT_SILU) v[e] = ex_act<YMK_ACT_SILU, sizeof(TO) == 2>(v[e]);
         else if (a.act == YMK_ACT_GELU) v[e] = ex_act<YMK_ACT_GELU, sizeof(TO) == 2>(v[e]);
         else if (a.act == YMK_ACT_SIGMOID) v[e] = ex_act<YMK_ACT_SIGMOID, sizeof(TO) == 2>(v[e]);
