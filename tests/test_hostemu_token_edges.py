@@ -1,5 +1,7 @@
 """Calls at the edges of what the token operators' wrappers accept, on the CPU lane emulator: operands that look right by their shape alone, empty
 batches of any rank, strides that do not fit the C interface, values that are not finite."""
+import warnings
+
 import pytest
 import torch
 
@@ -117,3 +119,28 @@ def test_rows_too_wide_for_the_kernels_counters(libs):
 @pytest.mark.parametrize("counts", [[2], [30, 9]])
 def test_scales_whose_product_is_subnormal(ops, counts):
     tc.check_product_small_scales(ops, counts)
+
+
+def test_operands_that_require_gradients(ops):
+    """Outputs carry no gradient: the forward calls say so where an operand asks for one, and are silent everywhere else."""
+    x, w, wt, off = torch.ones(4, 16), torch.ones(16), torch.ones(2, 8, 16), torch.tensor([0, 2, 4], dtype=torch.int32)
+    idx, gate = torch.tensor([[0], [1], [0], [1]], dtype=torch.int32), torch.ones(4, 1)
+    plan = ops.token_sort(idx, 2)
+    g = lambda t: t.clone().requires_grad_(True)   # noqa: E731
+    calls = [lambda f: ops.rms_norm(f(x), w), lambda f: ops.rms_norm(x, f(w), residual=x), lambda f: ops.rms_norm(x, w, residual=f(x)), lambda f: ops.rms_norm_quant(x, f(w)),
+             lambda f: ops.token_dispatch(f(x), plan), lambda f: ops.token_combine(x, plan, f(gate)), lambda f: ops.expert_linear(f(x), wt, off), lambda f: ops.expert_linear(x, f(wt), off),
+             lambda f: ops.expert_linear(x, wt, off, f(torch.ones(2, 8)))]
+    for call in calls:
+        with pytest.warns(UserWarning, match="requires gradients"):
+            out = call(g)
+        assert not (out[0] if isinstance(out, tuple) else out).requires_grad   # (rms_norm's h without a residual is x itself)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for call in calls:
+            call(lambda t: t)
+            with torch.no_grad():
+                call(g)
+        ops.rms_norm_backward(x, x, g(w), torch.ones(4))
+        ops.expert_linear_backward(torch.ones(4, 8), x, g(wt), off)
+        ops.token_combine_backward(x, x, plan, g(gate))
+        ops.token_dispatch_backward(x, plan)

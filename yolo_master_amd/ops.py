@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import os
+import warnings
 
 import torch
 
@@ -1192,7 +1193,7 @@ def tokens_to_rows(x, y, a_off: int, row_off: int = 0):
 # ----------------------------------------------------------------------------- tokens (include/ymk_tokens.h)
 # Rows instead of maps: [..., C] tensors whose last dim is dense and whose leading dims are one run of rows (any row stride >= C).  All operands of a
 # call live on the current device; outputs are new tensors of the current stream.  Gradients are calls of their own, for a training program's
-# autograd functions: these wrappers keep nothing between calls.
+# autograd functions: these wrappers keep nothing between calls, their outputs carry no gradient, and they warn where an operand asks for one.
 E4M3 = torch.float8_e4m3fn
 _ROW_DT = {**DT, E4M3: _lib.YMK_E4M3}
 _ROW_ACT = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "sigmoid": _lib.ACT_SIGMOID}
@@ -1246,9 +1247,14 @@ def _rows(t: torch.Tensor, what: str, most: int = 2**31 - 1):
 def _here(what: str, first: torch.Tensor, *others):
     """All operands on one GPU, and that the current one; its current stream, where the call goes."""
     dev = first.get_device()
+    wanted = first.requires_grad
     for t in others:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"{what}: operands on {first.device} and {t.device}")
+        if t is not None:
+            if t.get_device() != dev:
+                raise ValueError(f"{what}: operands on {first.device} and {t.device}")
+            wanted = wanted or t.requires_grad
+    if wanted and torch.is_grad_enabled() and not what.endswith("_backward"):
+        warnings.warn(f"{what}: an operand requires gradients, the outputs carry none: call it and its *_backward from an autograd function, or under torch.no_grad()", stacklevel=4)
     if dev < 0:
         require_gpu(first, what)
         return _stream()
