@@ -5,8 +5,8 @@
  * function says so), scales / gates / statistics fp32, `stream` a hipStream_t, return 0 or a negative YMK_E_* code, no allocation, no
  * synchronisation, no atomics on floating-point data: the same inputs give the same bits.  Every function may be captured into a graph;
  * a workspace belongs to the call (and, captured, to the graph) until the call has run.
- * Operands must lie on the current device; pointers and strides need the element type's alignment only (16-byte aligned rows take the
- * vectorised kernels) unless a function says more.  Zero rows: nothing is launched.
+ * Operands must lie on the current device; pointers and strides need the element type's alignment only (rows of any alignment take
+ * 16-byte accesses) unless a function says more.  Zero rows: nothing is launched.
  *
  * Gradients are calls of their own.
  *

@@ -12,11 +12,12 @@
 // a unit of a ring of five: the M side's unit of a step is brought during an earlier step's second half and the N side's during a first half, so that
 // transfers (and their LDS writes) go on evenly all the time, two to three halves ahead, with one barrier a step.
 //
-// Measured (MI355X; a large library product reaches 1440 TFLOP/s in bf16, 2710 in e4m3, 154 in fp32, a large copy 5.0-5.4 TB/s): 32768 rows over 8 experts,
-// 1024 -> 4096 in bf16: y 291 us (945 TFLOP/s), dx 308, dW and db 283; 4096 -> 4096: 924 us (1190); 65532 rows over 32 experts, 2048 -> 4096 in e4m3 with
-// SiLU 614 us (1790); other cards up to 6 % more.  What bounds it: the transfers (the loop without matrix instructions takes 0.85 of the whole, without transfers 0.8) and, where K is
-// short, the results' turn and the activation, which the one workgroup of a CU does not overlap with anything.  Workgroups that take tile after tile
-// and bring the next one's first step under the results of the last gained nothing (292 against 293 us, e4m3 778 against 568).
+// Measured (MI355X, two cards; a large library product reaches 1440 TFLOP/s in bf16, 2710 in e4m3, 154 in fp32, a large copy 5.0-5.4 TB/s): 32768 rows over 8
+// experts, 1024 -> 4096 in bf16: y 291-296 us (930-945 TFLOP/s), dx 308-315, dW and db 283-288; 4096 -> 4096: 872-924 us (1190-1260); 65532 rows over 32
+// experts, 2048 -> 4096 in e4m3 with SiLU 614-641 us (1720-1790).  What bounds it: the transfers (copies of the kernel without its matrix instructions took 0.85
+// of the whole, without its transfers 0.8) and, where K is short, the results' turn and the activation, which the one workgroup of a CU does not overlap with
+// anything.  Workgroups that take tile after tile and bring the next one's first step under the results of the last gained nothing (292 against 293 us,
+// e4m3 778 against 568).
 //
 // Fragments are those of the 32 x 32 matrix instructions: lane l holds row l % 32 and the 16-byte pieces l / 32 and 2 + l / 32 of a half's 64 bytes — the
 // order of K within a k-step is free as long as both sides use the same.  A side whose own index is contiguous is read through the transposing LDS
@@ -324,7 +325,7 @@ __device__ __forceinline__ float ex_act(float v) {
     } else return v;
 }
 
-// NKC / MKC: K contiguous on that side.  DW: K is the expert's rows.  TO: output type.
+// NKC / MKC: K contiguous on that side (of dW, whose K is the expert's rows, neither).  TO: output type.  DB: the sums of the M side's rows over K as well.
 template <typename T, typename TO, bool NKC, bool MKC, int TILE, bool DB>
 __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K, const char* nsrc, const char* msrc) {
     constexpr int WT = TILE / 64, UNIT = TILE * 128, LOADS = TILE / 32, CHUNKS = 2 * WT;
@@ -495,7 +496,7 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : TILE == 128 ? 2 : 4) void ex
 
 // y for few rows an expert: bound by the bytes of the experts' matrices.  A workgroup takes 16 rows by 32 channels; its four waves take the 128-byte pieces
 // of K in turn, EX_FEW_AHEAD of them in flight, straight from memory into the operands of the 16 x 16 matrix instructions (no LDS: nothing of W is used
-// twice), and add their sums up through LDS in the order of the waves.  8 tokens by two of 8 experts, 2048 -> 4096 in bf16: 26 us, 5.2 TB/s of weights.
+// twice), and add their sums up through LDS in the order of the waves.  8 tokens by two of 8 experts, 2048 -> 4096 in bf16: 27 us, 4.9 TB/s of weights.
 #define EX_FEW_N 32
 #define EX_FEW_AHEAD 4
 template <typename T>
@@ -648,16 +649,20 @@ inline int64_t ex_blocks(int64_t rows, int E, int N, int tm, int tn) {
     return (mt * nt + 7) / 8 * 8;
 }
 
-// Wider tiles bring fewer bytes to LDS for a product, but leave CUs idle when there are few of them and waste rows when experts have few.  Both sides, us:
+// Wider tiles bring fewer bytes to LDS for a product, but leave CUs idle when there are few of them and waste rows when experts have few.  Both sides, us a
+// call, the weights from memory (600 MB of them in turn):
 //     rows an expert   shape (16-bit unless said)              16     64    128    256
-//     1                6 rows of 64 experts, 4096 -> 2048 e4m3  9.4   12.9   16.9   39.6
-//     2                16 of 8, 2048 -> 4096                   24.1   23.2   24.0   46.7
-//     16               128 of 8, 2048 -> 4096                  36.6   24.3   25.4   44.6
-//     64               512 of 8, 2048 -> 4096                 100.5   31.9   28.5   47.4
-//     64               1024 of 16, 1024 -> 2048                60.2   16.3   16.7   27.9
-//     200              3202 of 16, 256 -> 520 fp32             31.3   18.9   23.9   70.3
-//     256              4096 of 16, 512 -> 2048                123.8   26.1   22.3   22.8
-//     4096             32768 of 8, 4096 -> 4096                              1159   1009
+//     1                6 rows of 64 experts, 4096 -> 2048 e4m3 16.0   21.5   22.3   39.4
+//     2                16 of 8, 2048 -> 4096                   29.7   34.7   34.8   43.3
+//     16               128 of 8, 2048 -> 4096                  31.3   35.0   35.0   43.1
+//     16               128 of 8, 2048 -> 4096 e4m3             17.8   17.5   15.7   24.0
+//     64               512 of 8, 2048 -> 4096                  91.7   35.3   37.0   45.5
+//     64               512 of 8, 2048 -> 4096 e4m3             52.7   19.3   17.7   26.3
+//     64               1024 of 16, 1024 -> 2048                52.7   16.9   17.2   26.0
+//     200              3202 of 16, 256 -> 520 fp32             27.9   18.4   22.9   69.2
+//     256              4096 of 16, 512 -> 2048                113.7   25.2   20.4   23.0
+//     4096             32768 of 8, 4096 -> 4096                              1099    886
+// The rule knows the average only: an expert that got most of the rows of a small call walks its matrix once per 16 of them.
 inline int ex_tile(int64_t rows, int E, int N) {
     auto tiles = [&](int tile) { return (rows / tile + E / 2) * ((N + tile - 1) / tile); };
     if (rows <= 16 || rows <= 4ll * E) return 16;
@@ -703,8 +708,9 @@ inline int64_t ex_dw_blocks(const ExArgs& a, int tile) {
 }
 template <typename T, typename TO>
 int ex_dw(const ExArgs& a, void* stream) {
-    // us at 64 / 128 / 256: 200 rows an expert, 16 of 520 x 256 fp32 18.9 / 31.0 / 88; 64 rows, 16 of 2048 x 1024 30.6 / 24.6 / 26.9; 256 rows, 16 of
-    // 2048 x 512 26.0 / 22.4 / 25.3; 4096 rows, 8 of 4096 x 1024 - / 353 / 318
+    // us at 64 / 128 / 256: 200 rows an expert, 16 of 520 x 256 fp32 18.3 / 25.5 / 65; 64 rows, 16 of 2048 x 1024 29.9 / 23.4 / 25.9; 256 rows, 16 of
+    // 2048 x 512 25.1 / 21.5 / 21.3; 4096 rows, 8 of 4096 x 4096 - / 1250 / 974.  K is not split: the workgroups are tiles times experts however many
+    // rows there are, so many rows over few small matrices leave CUs idle.
     const int tile = ex_forced() ? ex_forced() : a.rows >= 1024ll * a.E && ex_dw_blocks(a, 256) >= 512 ? 256 : ex_dw_blocks(a, 128) >= 512 ? 128 : 64;
     if (tile == 256) return ex_launch<expert_dw_kernel<T, TO, 256>>(a, ex_dw_blocks(a, 256), EX_UNITS * 256 * 128, stream);
     if (tile == 128) return ex_launch<expert_dw_kernel<T, TO, 128>>(a, ex_dw_blocks(a, 128), EX_UNITS * 128 * 128, stream);

@@ -5,7 +5,7 @@
 // (l + i * group) * V, so every load and store of a group is contiguous; V is 16 bytes (csrc/rows.h).  Groups of one wave
 // need no LDS and no barrier, so they take every width that fits their registers; wider rows are spread over a workgroup.
 // Measured: residual sum, norm and e4m3 output of 25600 x 2048 bf16 70 us (5.3 TB/s); of 4 x 4096 4.4 us; 102400 x 256 bf16 forward 36 us (5.8 TB/s), gradients
-// 37 + 5 us for dweight; 2041 x 1021 fp32 7.8 and 13 us (4.3 TB/s).
+// 37 + 5 us for dweight; 2041 x 1021 fp32 7.7 us (4.3 TB/s), gradients 10.3 + 3.8: one row a wave leaves 511 partial rows of dweight.
 #include "ymk_common.h"
 #include "rows.h"
 #include "../../include/ymk_tokens.h"
