@@ -6,7 +6,8 @@
  * synchronisation, no atomics on floating-point data: the same inputs give the same bits.  Every function may be captured into a graph;
  * a workspace belongs to the call (and, captured, to the graph) until the call has run.
  * Operands must lie on the current device; pointers and strides need the element type's alignment only (rows of any alignment take
- * 16-byte accesses) unless a function says more.  Zero rows: nothing is launched.
+ * 16-byte accesses) unless a function says more.  Zero rows: only what does not lie in rows is written (a sort's offsets; dweight, dW and
+ * db: zeros).
  *
  * Gradients are calls of their own.
  *

@@ -1,6 +1,10 @@
 """Calls at the edges of what the token operators' wrappers accept, on the CPU lane emulator: operands that look right by their shape alone, empty
 batches of any rank, strides that do not fit the C interface, values that are not finite."""
+import os
+import subprocess
+import sys
 import warnings
+from pathlib import Path
 
 import pytest
 import torch
@@ -144,3 +148,24 @@ def test_operands_that_require_gradients(ops):
         ops.expert_linear_backward(torch.ones(4, 8), x, g(wt), off)
         ops.token_combine_backward(x, x, plan, g(gate))
         ops.token_dispatch_backward(x, plan)
+
+
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
+def test_8bit_products_with_16bit_outputs_at_every_tile(tile, libs):
+    """The switch is read once a process."""
+    code = (
+        "import torch, ctypes as C\n"
+        "from tests import token_cases as tc\n"
+        "from tests.hostemu import build\n"
+        "from yolo_master_amd import _lib, ops\n"
+        "h = C.CDLL(str(build.build()))\n"
+        "for name, (res, args) in _lib.SYMBOLS_TOKENS.items(): fn = getattr(h, name); fn.restype, fn.argtypes = res, args\n"
+        "ops.lib, ops._stream, ops.require_gpu = h, lambda: None, lambda t, what='': None\n"
+        "for c in (([130, 0, 1, 37], 80, 144), ([5, 129], 208, 16)): tc.check_product_exact_16(ops, *c, torch.bfloat16)\n"
+        "tc.check_product(ops, torch.float8_e4m3fn, ([70, 0, 3], 1, 144, 40, 'gelu', 16))\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=str(Path(__file__).resolve().parent.parent), env={**os.environ, "YMK_EXPERT_TILE": tile}, timeout=600)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_norm_over_its_own_inputs(ops, dtype):
+    tc.check_norm_aliases(ops, dtype)

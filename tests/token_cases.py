@@ -544,3 +544,44 @@ def check_product_small_scales(ops, counts, dev="cpu"):
     for dtype in (torch.float32, torch.bfloat16):
         y = ops.expert_linear(x.to(dev), w.to(dev), make_offsets(counts).to(dev), x_scale=xs.to(dev), w_scale=ws.to(dev), out_dtype=dtype)
         close(y, torch.full((rows, Cout), want, dtype=torch.float64), torch.full((rows, Cout), want * (half(dtype) + (Cin + 8) * U)), "small scales")
+
+
+def check_product_exact_16(ops, counts, Cin, Cout, out_dtype, dev="cpu"):
+    """check_product_exact with a 16-bit output: products span 10 bits, fewer than the 8-bit instruction keeps, so the output is the exact sum rounded once."""
+    g = gen(Cin * 3 + Cout)
+    E, rows = len(counts), sum(counts) + 2
+    pick = lambda *s: (torch.randint(8, 16, s, generator=g) * torch.tensor([0.125, 0.25, -0.25])[torch.randint(0, 3, s, generator=g)]).to(torch.float8_e4m3fn)   # noqa: E731
+    x, w = pick(rows, Cin), pick(E, Cout, Cin)
+    xs, ws = 2.0 ** torch.randint(-3, 3, (rows,), generator=g).float(), 2.0 ** torch.randint(-3, 3, (E, Cout), generator=g).float()
+    off = make_offsets(counts)
+    y = ops.expert_linear(x.to(dev), w.to(dev), off.to(dev), x_scale=xs.to(dev), w_scale=ws.to(dev), out_dtype=out_dtype).cpu()
+    for e, n in enumerate(counts):
+        s = slice(int(off[e]), int(off[e]) + n)
+        want = (x[s].to(dev).double() @ w[e].to(dev).double().t()).cpu() * xs[s].double()[:, None] * ws[e].double()
+        assert torch.equal(y[s], want.to(out_dtype)), e
+
+
+def check_norm_aliases(ops, dtype, dev="cpu"):
+    """The C functions' outputs over their inputs, same stride: y over x or residual beside h over the other one, codes apart; dx over dy, h and dres."""
+    g = gen(41)
+    dt, s, lib = ops.DT[dtype], ops._stream(), ops._lib_for(dtype)
+    for M, C, pad in ((5, 3, 0), (7, 37, 5), (9, 40, 0), (70, 64, 8), (3, 1021, 2), (6, 2100, 0)):
+        ld = C + pad
+        new = lambda: rows_of(g, M, C, dtype, pad, dev)   # noqa: E731
+        x, r, w = new(), new(), (1 + 0.1 * torch.randn(C, generator=g)).to(dev)
+        y, h, rstd = ops.rms_norm(x, w, residual=r)
+        copy = lambda t: torch.empty(M, ld, dtype=dtype, device=dev)[:, :C].copy_(t)   # noqa: E731
+        for swap in (False, True):
+            a, b = copy(x), copy(r)
+            ho, yo = (b, a) if swap else (a, b)
+            assert lib.ymk_rms_norm(dt, a.data_ptr(), ld, b.data_ptr(), ld, ho.data_ptr(), ld, yo.data_ptr(), ld, None, M, C, w.data_ptr(), 1e-6, s) == 0
+            assert torch.equal(ho, h) and torch.equal(yo, y), (C, swap)
+        a = copy(x)
+        assert lib.ymk_rms_norm(dt, a.data_ptr(), ld, None, 0, None, 0, a.data_ptr(), ld, None, M, C, w.data_ptr(), 1e-6, s) == 0
+        assert torch.equal(a, ops.rms_norm(x, w)[0])
+        dy, dres = new(), new()
+        dx, _ = ops.rms_norm_backward(dy, h, w, rstd, dres=dres, need_dweight=False)
+        for i in range(3):
+            t = [copy(v) for v in (dy, h, dres)]
+            assert lib.ymk_rms_norm_backward(dt, t[0].data_ptr(), ld, t[1].data_ptr(), ld, rstd.data_ptr(), w.data_ptr(), t[2].data_ptr(), ld, t[i].data_ptr(), ld, None, M, C, None, 0, s) == 0
+            assert torch.equal(t[i], dx), (C, i)

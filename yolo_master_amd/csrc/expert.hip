@@ -671,7 +671,8 @@ inline int ex_tile(int64_t rows, int E, int N) {
     return 64;
 }
 
-// A/B and test switch, read at first use: YMK_EXPERT_TILE=16|64|128|256 takes that tile for every size (16: y only; the others then take 64)
+// A/B and test switch, read at first use: YMK_EXPERT_TILE=16|64|128|256 takes that tile for every size (16: y only, the others then take 64; 256: 8-bit
+// rows with an fp32 output take 128)
 inline int ex_forced() {
     static const int tile = [] {
         const char* s = getenv("YMK_EXPERT_TILE");
