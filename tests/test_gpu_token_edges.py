@@ -69,3 +69,12 @@ def test_8bit_products_with_16bit_outputs_at_every_tile(tile):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_norm_over_its_own_inputs(ops, dtype):
     tc.check_norm_aliases(ops, dtype, DEV)
+
+
+def test_bias_sums(ops):
+    tc.check_long_bias_sums(ops, torch.float32, [12000, 0, 31], 1.0001, DEV)
+    tc.check_long_bias_sums(ops, torch.float32, [100003, 40000], 1.0001, DEV)
+    for dtype, value in ((torch.bfloat16, 1 + 2.0**-7), (torch.float16, 1 + 2.0**-10)):
+        tc.check_long_bias_sums(ops, dtype, [700001, 33], value, DEV)
+    for dtype in DTYPES:
+        tc.check_bias_sums_that_are_not_finite(ops, dtype, DEV)

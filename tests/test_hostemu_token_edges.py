@@ -169,3 +169,10 @@ def test_8bit_products_with_16bit_outputs_at_every_tile(tile, libs):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_norm_over_its_own_inputs(ops, dtype):
     tc.check_norm_aliases(ops, dtype)
+
+
+def test_bias_sums(ops):
+    tc.check_long_bias_sums(ops, torch.float32, [12000, 0, 31], 1.0001)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        tc.check_long_bias_sums(ops, dtype, [100, 1, 64], 1.0)
+        tc.check_bias_sums_that_are_not_finite(ops, dtype)

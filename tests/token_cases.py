@@ -585,3 +585,29 @@ def check_norm_aliases(ops, dtype, dev="cpu"):
             t = [copy(v) for v in (dy, h, dres)]
             assert lib.ymk_rms_norm_backward(dt, t[0].data_ptr(), ld, t[1].data_ptr(), ld, rstd.data_ptr(), w.data_ptr(), t[2].data_ptr(), ld, t[i].data_ptr(), ld, None, M, C, None, 0, s) == 0
             assert torch.equal(t[i], dx), (C, i)
+
+
+def check_long_bias_sums(ops, dtype, counts, value, dev="cpu"):
+    """db of many rows of one value, where a running fp32 sum grows until each addition loses the value's last bits.  A fragment of up to 16 values is added as
+    a tree (4 levels, each off by half a step of 2^-23), the fragments' sums with their rounding errors kept: 8 u of the sum of magnitudes is ample."""
+    E, Cin, Cout = len(counts), 16 // torch.empty(0, dtype=dtype).element_size(), 8
+    rows = sum(counts)
+    x, dy = torch.ones(rows, Cin, dtype=dtype, device=dev), torch.full((rows, Cout), value, device=dev).to(dtype)
+    dy[:, 1::2] *= -1
+    _, _, db = ops.expert_linear_backward(dy, x, torch.ones(E, Cout, Cin, dtype=dtype, device=dev), make_offsets(counts).to(dev), need_dx=False)
+    want = torch.tensor(counts, dtype=torch.float64)[:, None] * dy[:1].double().cpu()
+    close(db, want, want.abs() * (8 * U), "db")
+
+
+def check_bias_sums_that_are_not_finite(ops, dtype, dev="cpu"):
+    inf, nan = float("inf"), float("nan")
+    n, Cin, Cout = 300, 8, 8
+    dy = torch.ones(n, Cout, dtype=dtype)
+    dy[70, 0], dy[3, 1], dy[5, 2], dy[250, 3], dy[40, 3], dy[:, 4] = inf, -inf, nan, inf, -inf, torch.finfo(dtype).max
+    x = torch.ones(n, Cin, dtype=dtype)
+    _, _, db = ops.expert_linear_backward(dy.to(dev), x.to(dev), torch.ones(1, Cout, Cin, dtype=dtype, device=dev), make_offsets([n]).to(dev), need_dx=False)
+    want = dy.double().sum(0).float()
+    db = db[0].cpu()
+    assert torch.equal(torch.isnan(db), torch.isnan(want)) and torch.equal(db[torch.isinf(want)], want[torch.isinf(want)]), (db, want)
+    f = torch.isfinite(want)
+    close(db[f], want[f], want[f].double().abs() * (8 * U), "db")

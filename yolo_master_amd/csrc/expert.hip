@@ -123,18 +123,24 @@ __device__ __forceinline__ f32x16 ex_mfma(const ExFrag& a, const ExFrag& b, f32x
     }
 }
 
-// c + the elements of a fragment
+// the elements of a fragment, added as a tree
 template <typename T>
-__device__ __forceinline__ float ex_sum(const ExFrag& f, float c) {
+__device__ __forceinline__ float ex_sum(const ExFrag& f) {
+    float s[4];
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t w = f.p[q][i];
-            if constexpr (sizeof(T) == 4) c += __uint_as_float(w);
-            else c = dot2_h16(w, pack_h16x2(1.f, 1.f), c);
-        }
-    return c;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = f.p[i >> 1][(i & 1) * 2], b = f.p[i >> 1][(i & 1) * 2 + 1];
+        if constexpr (sizeof(T) == 4) s[i] = __uint_as_float(a) + __uint_as_float(b);
+        else s[i] = dot2_h16(b, pack_h16x2(1.f, 1.f), dot2_h16(a, pack_h16x2(1.f, 1.f), 0.f));
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+// hi + v with its rounding error added to lo (the two-sum of Knuth, The Art of Computer Programming 2, 4.2.2): K of db is the expert's rows, and a running
+// sum of 12617 normal values in fp32 was four times as far off as one added in blocks
+__device__ __forceinline__ void ex_add(float& hi, float& lo, float v) {
+    const float t = hi + v, w = t - hi;
+    lo += (hi - (t - w)) + (v - w);
+    hi = t;
 }
 
 // A raw buffer at p (an offset with bit 31 set is out of its range: zeros, no access), and 16 bytes a lane from it to LDS at dst (wave-uniform) + lane * 16.
@@ -353,7 +359,7 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
         mscale[j] = a.m_scale && row < t.mend ? a.m_scale[row] : 1.f;
     }
     f32x16 acc[WT][WT];
-    float accb[WT];   // DB: this lane's part of the sum over K of its M-side rows
+    float accb[WT], lowb[WT];   // DB: this lane's part of the sum over K of its M-side rows, and what its additions rounded off
 #pragma unroll
     for (int i = 0; i < WT; ++i)
 #pragma unroll
@@ -361,7 +367,7 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 #pragma unroll
-    for (int j = 0; j < WT; ++j) accb[j] = 0.f;
+    for (int j = 0; j < WT; ++j) accb[j] = lowb[j] = 0.f;
     ExFrag fn[2][WT], fm[2][WT];   // the fragments of a step's two halves
     const int steps = (K + NSide::KS - 1) / NSide::KS;
     // Units in the order they are brought: N of step 0, M of step 0, N of 1, ...; unit u lies at (u % 5) * UNIT.  Step k's are free once every wave has the
@@ -406,7 +412,7 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
             }
             if (c < WT) {
                 fn[1 - h][c] = NSide::read(nsrc_, (wn * WT + c) * 32, 1 - h, lane);
-                if constexpr (DB) accb[c] = ex_sum<T>(fm[h][c], accb[c]);
+                if constexpr (DB) ex_add(accb[c], lowb[c], ex_sum<T>(fm[h][c]));
             } else {
                 fm[1 - h][c - WT] = MSide::read(msrc_, (wm * WT + c - WT) * 32, 1 - h, lane);
             }
@@ -439,7 +445,10 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
         if (row0 >= t.mend) break;
         if constexpr (DB) {
             const int row = row0 + (MKC ? lane & 31 : ex_perm(lane & 31));
-            const float sum = accb[j] + __shfl_xor(accb[j], 32);   // lanes l and l + 32 hold the same row's other halves of K
+            float sum = accb[j], low = lowb[j];   // lanes l and l + 32 hold the same row's other halves of K
+            ex_add(sum, low, __shfl_xor(accb[j], 32));
+            low += __shfl_xor(lowb[j], 32);
+            sum = fabsf(sum) < __uint_as_float(0x7f800000u) ? sum + low : sum;   // what an infinite sum rounds off is no number
             if (wn == 0 && h == 0 && row < t.mend) a.db[(int64_t)t.e * a.M + row] = sum;
         }
         float* w = turn + (MKC ? lane & 31 : ex_perm(lane & 31)) * LD + h * 16;
