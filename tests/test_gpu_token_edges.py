@@ -78,3 +78,8 @@ def test_bias_sums(ops):
         tc.check_long_bias_sums(ops, dtype, [700001, 33], value, DEV)
     for dtype in DTYPES:
         tc.check_bias_sums_that_are_not_finite(ops, dtype, DEV)
+
+
+def test_weight_gradients_of_many_rows(ops):
+    tc.check_long_weight_sums(ops, torch.float32, [12000, 0, 511, 513], 1.0001, DEV)
+    tc.check_long_weight_sums(ops, torch.float32, [100003, 512], 1.0001, DEV)

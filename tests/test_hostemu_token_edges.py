@@ -176,3 +176,7 @@ def test_bias_sums(ops):
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
         tc.check_long_bias_sums(ops, dtype, [100, 1, 64], 1.0)
         tc.check_bias_sums_that_are_not_finite(ops, dtype)
+
+
+def test_weight_gradients_of_many_rows(ops):
+    tc.check_long_weight_sums(ops, torch.float32, [12000, 0, 511, 513], 1.0001)

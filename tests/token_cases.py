@@ -611,3 +611,16 @@ def check_bias_sums_that_are_not_finite(ops, dtype, dev="cpu"):
     assert torch.equal(torch.isnan(db), torch.isnan(want)) and torch.equal(db[torch.isinf(want)], want[torch.isinf(want)]), (db, want)
     f = torch.isfinite(want)
     close(db[f], want[f], want[f].double().abs() * (8 * U), "db")
+
+
+def check_long_weight_sums(ops, dtype, counts, value, dev="cpu", dw_dtype=None):
+    """dW of many rows of one value: blocks of 512 rows are chains of 256 additions (of two products each) or fewer, the blocks a chain of their own; each addition is
+    off by half a step of the running sum.  One chain over all the rows would lose the value's last bits at every step."""
+    E, Cin, Cout = len(counts), 24, 40
+    rows = sum(counts)
+    x, dy = torch.ones(rows, Cin, dtype=dtype, device=dev), torch.full((rows, Cout), value, device=dev).to(dtype)
+    dy[:, 1::2] *= -1
+    _, dw, _ = ops.expert_linear_backward(dy, x, torch.ones(E, Cout, Cin, dtype=dtype, device=dev), make_offsets(counts).to(dev), need_dx=False, dw_dtype=dw_dtype)
+    for e, n in enumerate(counts):
+        want = (n * dy[0].double().cpu())[:, None].expand(Cout, Cin)
+        close(dw[e], want, want.abs() * ((256 + n // 512 + 8) * U + (half(dw.dtype) if dw.dtype != torch.float32 else 0.0)), f"dw {e}")

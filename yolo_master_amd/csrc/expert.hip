@@ -136,7 +136,7 @@ __device__ __forceinline__ float ex_sum(const ExFrag& f) {
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 // hi + v with its rounding error added to lo (the two-sum of Knuth, The Art of Computer Programming 2, 4.2.2): K of db is the expert's rows, and a running
-// sum of 12617 normal values in fp32 was four times as far off as one added in blocks
+// sum of 12617 normal values in fp32 was 1.4e-6 off, this one 5e-8
 __device__ __forceinline__ void ex_add(float& hi, float& lo, float v) {
     const float t = hi + v, w = t - hi;
     lo += (hi - (t - w)) + (v - w);
@@ -368,6 +368,30 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 #pragma unroll
     for (int j = 0; j < WT; ++j) accb[j] = lowb[j] = 0.f;
+    // K of an fp32 dW is the expert's rows, two of them a matrix instruction: every 512 rows the accumulators go into sums of their own, so that no chain of
+    // additions is longer than 256 or the number of such blocks (53499 rows of normal values: 4.5e-7 off
+    // relative to the result, 4.1e-6 as one chain, 3 % of the time).  16-bit inputs add 16 rows an instruction.
+    constexpr bool FOLD = std::is_same<T, float>::value && !NKC && !MKC;
+    f32x16 far[FOLD ? WT : 1][FOLD ? WT : 1];
+    if constexpr (FOLD) {
+#pragma unroll
+        for (int i = 0; i < WT; ++i)
+#pragma unroll
+            for (int j = 0; j < WT; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) far[i][j][r] = 0.f;
+    }
+    auto fold = [&] {
+#pragma unroll
+        for (int i = 0; i < WT; ++i)
+#pragma unroll
+            for (int j = 0; j < WT; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    far[i][j][r] += acc[i][j][r];
+                    acc[i][j][r] = 0.f;
+                }
+    };
     ExFrag fn[2][WT], fm[2][WT];   // the fragments of a step's two halves
     const int steps = (K + NSide::KS - 1) / NSide::KS;
     // Units in the order they are brought: N of step 0, M of step 0, N of 1, ...; unit u lies at (u % 5) * UNIT.  Step k's are free once every wave has the
@@ -427,6 +451,16 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
         GLDS_COMPILER_FENCE();
         half(std::integral_constant<int, 1>{}, unit(un + 2), unit(un + 3), unit(un), ms.at(k + 2));
         un = un + 2 >= EX_UNITS ? un + 2 - EX_UNITS : un + 2;
+        if constexpr (FOLD) {
+            if ((k & 15) == 15) fold();
+        }
+    }
+    if constexpr (FOLD) {
+        fold();
+#pragma unroll
+        for (int i = 0; i < WT; ++i)
+#pragma unroll
+            for (int j = 0; j < WT; ++j) acc[i][j] = far[i][j];
     }
     __builtin_amdgcn_s_waitcnt(GLDS_WAITCNT_VM(0));   // the transfers of zeros behind the last step have landed: LDS is free once every wave is here
     __syncthreads();
@@ -681,7 +715,7 @@ inline int ex_tile(int64_t rows, int E, int N) {
 }
 
 // A/B and test switch, read at first use: YMK_EXPERT_TILE=16|64|128|256 takes that tile for every size (16: y only, the others then take 64; 256: 8-bit
-// rows with an fp32 output take 128)
+// rows with an fp32 output and an fp32 dW take 128)
 inline int ex_forced() {
     static const int tile = [] {
         const char* s = getenv("YMK_EXPERT_TILE");
@@ -722,8 +756,11 @@ int ex_dw(const ExArgs& a, void* stream) {
     // 2048 x 512 25.1 / 21.5 / 21.3; 4096 rows, 8 of 4096 x 4096 - / 1250 / 974.  K is not split: the workgroups are tiles times experts however many
     // rows there are, so many rows over few small matrices leave CUs idle.
     const int tile = ex_forced() ? ex_forced() : a.rows >= 1024ll * a.E && ex_dw_blocks(a, 256) >= 512 ? 256 : ex_dw_blocks(a, 128) >= 512 ? 128 : 64;
-    if (tile == 256) return ex_launch<expert_dw_kernel<T, TO, 256>>(a, ex_dw_blocks(a, 256), EX_UNITS * 256 * 128, stream);
-    if (tile == 128) return ex_launch<expert_dw_kernel<T, TO, 128>>(a, ex_dw_blocks(a, 128), EX_UNITS * 128 * 128, stream);
+    // Two sets of fp32 accumulators of 256 x 256 do not fit the registers; 128 is as fast there: 4096 rows, 8 of 4096 x 1024 2049 / 2056 us at 256 / 128 before
+    if constexpr (!std::is_same<T, float>::value) {
+        if (tile == 256) return ex_launch<expert_dw_kernel<T, TO, 256>>(a, ex_dw_blocks(a, 256), EX_UNITS * 256 * 128, stream);
+    }
+    if (tile >= 128) return ex_launch<expert_dw_kernel<T, TO, 128>>(a, ex_dw_blocks(a, 128), EX_UNITS * 128 * 128, stream);
     return ex_launch<expert_dw_kernel<T, TO, 64>>(a, ex_dw_blocks(a, 64), EX_UNITS * 64 * 128, stream);
 }
 
