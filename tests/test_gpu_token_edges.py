@@ -83,3 +83,8 @@ def test_bias_sums(ops):
 def test_weight_gradients_of_many_rows(ops):
     tc.check_long_weight_sums(ops, torch.float32, [12000, 0, 511, 513], 1.0001, DEV)
     tc.check_long_weight_sums(ops, torch.float32, [100003, 512], 1.0001, DEV)
+
+
+@pytest.mark.parametrize("rows,K", [(30, 20000), (200, 100000), (2, 100000)])
+def test_products_of_many_channels(ops, rows, K):
+    tc.check_long_products(ops, rows, K, DEV)

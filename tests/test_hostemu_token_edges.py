@@ -180,3 +180,8 @@ def test_bias_sums(ops):
 
 def test_weight_gradients_of_many_rows(ops):
     tc.check_long_weight_sums(ops, torch.float32, [12000, 0, 511, 513], 1.0001)
+
+
+def test_products_of_many_channels(ops):
+    tc.check_long_products(ops, 30, 20000)
+    tc.check_long_products(ops, 2, 60000)

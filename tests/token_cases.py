@@ -624,3 +624,14 @@ def check_long_weight_sums(ops, dtype, counts, value, dev="cpu", dw_dtype=None):
     for e, n in enumerate(counts):
         want = (n * dy[0].double().cpu())[:, None].expand(Cout, Cin)
         close(dw[e], want, want.abs() * ((256 + n // 512 + 8) * U + (half(dw.dtype) if dw.dtype != torch.float32 else 0.0)), f"dw {e}")
+
+
+def check_long_products(ops, rows, K, dev="cpu"):
+    """y and dx in fp32 over K channels of one value, as check_long_weight_sums does with rows."""
+    off = make_offsets([rows, 0, 1]).to(dev)
+    one, many = torch.ones(rows + 1, K, device=dev), torch.full((3, 8, K), 1.0001, device=dev)
+    y = ops.expert_linear(one, many, off)
+    dx, _, _ = ops.expert_linear_backward(one, torch.ones(rows + 1, 8, device=dev), many.transpose(1, 2).contiguous(), off, need_dw=False, need_db=False)
+    want = torch.full((rows + 1, 8), K, dtype=torch.float64) * float(many[0, 0, 0])
+    for got, what in ((y, "y"), (dx, "dx")):
+        close(got, want, want * ((256 + K // 512 + 8) * U), what)

@@ -368,10 +368,10 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 #pragma unroll
     for (int j = 0; j < WT; ++j) accb[j] = lowb[j] = 0.f;
-    // K of an fp32 dW is the expert's rows, two of them a matrix instruction: every 512 rows the accumulators go into sums of their own, so that no chain of
-    // additions is longer than 256 or the number of such blocks (53499 rows of normal values: 4.5e-7 off
-    // relative to the result, 4.1e-6 as one chain, 3 % of the time).  16-bit inputs add 16 rows an instruction.
-    constexpr bool FOLD = std::is_same<T, float>::value && !NKC && !MKC;
+    // An fp32 matrix instruction adds two products: every 512 of K the accumulators go into sums of their own, so that no chain of additions is longer than
+    // 256 or the number of such blocks.  dW, whose K is the expert's rows, of 53499 rows of normal values: 4.5e-7 off relative to the result, 4.1e-6 as one
+    // chain; y of 4096 channels 4.1e-7 and 1.15e-6.  The accumulators of 256 x 256 leave no registers for it.  16-bit operands come 16 an instruction.
+    constexpr bool FOLD = std::is_same<T, float>::value && TILE <= 128;
     f32x16 far[FOLD ? WT : 1][FOLD ? WT : 1];
     if constexpr (FOLD) {
 #pragma unroll
@@ -595,6 +595,10 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ExArgs a) {
         f.p[1] = *reinterpret_cast<const u32x4*>(p + at + 64 + piece);
         return f;
     };
+    constexpr bool FOLD = std::is_same<T, float>::value;   // as in ex_body, every 128 of K (32 additions of four products)
+    f32x4 far[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) far[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     int k = wave;
     for (; k + 4 * (EX_FEW_AHEAD - 1) < full; k += 4 * EX_FEW_AHEAD) {
         ExFrag x[EX_FEW_AHEAD], w[EX_FEW_AHEAD][NB];
@@ -609,6 +613,13 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ExArgs a) {
         for (int u = 0; u < EX_FEW_AHEAD; ++u)
 #pragma unroll
             for (int i = 0; i < NB; ++i) acc[i] = ex_mfma16<T>(w[u][i], x[u], acc[i]);
+        if constexpr (FOLD) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                far[i] += acc[i];
+                acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
     }
     for (; k < full; k += 4) {
         const ExFrag x = load(xp, k * 128);
@@ -633,7 +644,7 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ExArgs a) {
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) part[wave][r][i * 16 + (lane >> 4) * 4 + q] = acc[i][q];
+        for (int q = 0; q < 4; ++q) part[wave][r][i * 16 + (lane >> 4) * 4 + q] = FOLD ? far[i][q] + acc[i][q] : acc[i][q];
     __syncthreads();
     if (t.m0 + ((int)threadIdx.x >> 4) >= t.mend || c >= a.N) return;
     float v[2];
