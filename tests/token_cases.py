@@ -588,15 +588,16 @@ def check_norm_aliases(ops, dtype, dev="cpu"):
 
 
 def check_long_bias_sums(ops, dtype, counts, value, dev="cpu"):
-    """db of many rows of one value, where a running fp32 sum grows until each addition loses the value's last bits.  A fragment of up to 16 values is added as
-    a tree (4 levels, each off by half a step of 2^-23), the fragments' sums with their rounding errors kept: 8 u of the sum of magnitudes is ample."""
+    """db of many rows of one value, where a running fp32 sum grows until each addition loses the value's last bits.  Four steps of a lane are a chain of 64
+    additions (of two 16-bit values at a time, one rounding each), each off by at most u of the sum of magnitudes so far; these sums are added with their rounding
+    errors kept, which leaves a few u: 64 + 8."""
     E, Cin, Cout = len(counts), 16 // torch.empty(0, dtype=dtype).element_size(), 8
     rows = sum(counts)
     x, dy = torch.ones(rows, Cin, dtype=dtype, device=dev), torch.full((rows, Cout), value, device=dev).to(dtype)
     dy[:, 1::2] *= -1
     _, _, db = ops.expert_linear_backward(dy, x, torch.ones(E, Cout, Cin, dtype=dtype, device=dev), make_offsets(counts).to(dev), need_dx=False)
     want = torch.tensor(counts, dtype=torch.float64)[:, None] * dy[:1].double().cpu()
-    close(db, want, want.abs() * (8 * U), "db")
+    close(db, want, want.abs() * (72 * U), "db")
 
 
 def check_bias_sums_that_are_not_finite(ops, dtype, dev="cpu"):
@@ -610,7 +611,7 @@ def check_bias_sums_that_are_not_finite(ops, dtype, dev="cpu"):
     db = db[0].cpu()
     assert torch.equal(torch.isnan(db), torch.isnan(want)) and torch.equal(db[torch.isinf(want)], want[torch.isinf(want)]), (db, want)
     f = torch.isfinite(want)
-    close(db[f], want[f], want[f].double().abs() * (8 * U), "db")
+    close(db[f], want[f], want[f].double().abs() * (72 * U), "db")
 
 
 def check_long_weight_sums(ops, dtype, counts, value, dev="cpu", dw_dtype=None):

@@ -123,20 +123,22 @@ __device__ __forceinline__ f32x16 ex_mfma(const ExFrag& a, const ExFrag& b, f32x
     }
 }
 
-// the elements of a fragment, added as a tree
+// c + the elements of a fragment
 template <typename T>
-__device__ __forceinline__ float ex_sum(const ExFrag& f) {
-    float s[4];
+__device__ __forceinline__ float ex_sum(const ExFrag& f, float c) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t a = f.p[i >> 1][(i & 1) * 2], b = f.p[i >> 1][(i & 1) * 2 + 1];
-        if constexpr (sizeof(T) == 4) s[i] = __uint_as_float(a) + __uint_as_float(b);
-        else s[i] = dot2_h16(b, pack_h16x2(1.f, 1.f), dot2_h16(a, pack_h16x2(1.f, 1.f), 0.f));
-    }
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = f.p[q][i];
+            if constexpr (sizeof(T) == 4) c += __uint_as_float(w);
+            else c = dot2_h16(w, pack_h16x2(1.f, 1.f), c);
+        }
+    return c;
 }
-// hi + v with its rounding error added to lo (the two-sum of Knuth, The Art of Computer Programming 2, 4.2.2): K of db is the expert's rows, and a running
-// sum of 12617 normal values in fp32 was 1.4e-6 off, this one 5e-8
+// hi + v with its rounding error added to lo (the two-sum of Knuth, The Art of Computer Programming 2, 4.2.2).  K of db is the expert's rows: as one running
+// sum, 12617 normal values in fp32 were 1.4e-6 off.  Four steps (64 additions of one value, or of two 16-bit ones) are a sum of their own, which goes into
+// hi and lo: 1.5e-7.  (Every fragment into hi and lo took dW and db of 32768 rows over 8 experts, 1024 -> 4096 in bf16 from 264 to 287 us, this costs nothing.)
 __device__ __forceinline__ void ex_add(float& hi, float& lo, float v) {
     const float t = hi + v, w = t - hi;
     lo += (hi - (t - w)) + (v - w);
@@ -359,7 +361,7 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
         mscale[j] = a.m_scale && row < t.mend ? a.m_scale[row] : 1.f;
     }
     f32x16 acc[WT][WT];
-    float accb[WT], lowb[WT];   // DB: this lane's part of the sum over K of its M-side rows, and what its additions rounded off
+    float accb[WT], sumb[WT], lowb[WT];   // DB: this lane's part of the sum over K of its M-side rows: the last steps', those before, and what their sum rounded off
 #pragma unroll
     for (int i = 0; i < WT; ++i)
 #pragma unroll
@@ -367,7 +369,7 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 #pragma unroll
-    for (int j = 0; j < WT; ++j) accb[j] = lowb[j] = 0.f;
+    for (int j = 0; j < WT; ++j) accb[j] = sumb[j] = lowb[j] = 0.f;
     // An fp32 matrix instruction adds two products: every 512 of K the accumulators go into sums of their own, so that no chain of additions is longer than
     // 256 or the number of such blocks.  dW, whose K is the expert's rows, of 53499 rows of normal values: 4.5e-7 off relative to the result, 4.1e-6 as one
     // chain; y of 4096 channels 4.1e-7 and 1.15e-6.  The accumulators of 256 x 256 leave no registers for it.  16-bit operands come 16 an instruction.
@@ -436,7 +438,7 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
             }
             if (c < WT) {
                 fn[1 - h][c] = NSide::read(nsrc_, (wn * WT + c) * 32, 1 - h, lane);
-                if constexpr (DB) ex_add(accb[c], lowb[c], ex_sum<T>(fm[h][c]));
+                if constexpr (DB) accb[c] = ex_sum<T>(fm[h][c], accb[c]);
             } else {
                 fm[1 - h][c - WT] = MSide::read(msrc_, (wm * WT + c - WT) * 32, 1 - h, lane);
             }
@@ -453,6 +455,15 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
         un = un + 2 >= EX_UNITS ? un + 2 - EX_UNITS : un + 2;
         if constexpr (FOLD) {
             if ((k & 15) == 15) fold();
+        }
+        if constexpr (DB) {
+            if ((k & 3) == 3 || k == steps - 1) {
+#pragma unroll
+                for (int j = 0; j < WT; ++j) {
+                    ex_add(sumb[j], lowb[j], accb[j]);
+                    accb[j] = 0.f;
+                }
+            }
         }
     }
     if constexpr (FOLD) {
@@ -479,8 +490,8 @@ __device__ __forceinline__ void ex_body(const ExArgs& a, const ExTile& t, int K,
         if (row0 >= t.mend) break;
         if constexpr (DB) {
             const int row = row0 + (MKC ? lane & 31 : ex_perm(lane & 31));
-            float sum = accb[j], low = lowb[j];   // lanes l and l + 32 hold the same row's other halves of K
-            ex_add(sum, low, __shfl_xor(accb[j], 32));
+            float sum = sumb[j], low = lowb[j];   // lanes l and l + 32 hold the same row's other halves of K
+            ex_add(sum, low, __shfl_xor(sumb[j], 32));
             low += __shfl_xor(lowb[j], 32);
             sum = fabsf(sum) < __uint_as_float(0x7f800000u) ? sum + low : sum;   // what an infinite sum rounds off is no number
             if (wn == 0 && h == 0 && row < t.mend) a.db[(int64_t)t.e * a.M + row] = sum;
